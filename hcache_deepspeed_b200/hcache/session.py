@@ -11,7 +11,7 @@ from typing import Callable, Dict, List, Optional
 
 import torch
 
-from ..inference.sampling import sample_next
+from ..inference.sampling import LogitControls, sample_next
 from .planner import LinkModel, RestorePlan, measure_link, plan_restore
 from .store import HiddenStateStore, SessionState
 
@@ -70,21 +70,25 @@ class HCacheSessionManager:
 
     def decode(self, uids: List[int], max_new_tokens: int, first_logits: torch.Tensor, do_sample: bool = False,
                temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
-               stop: Optional[Callable[[int, int], bool]] = None) -> List[List[int]]:
-        """Batched decode of resident sessions. ``first_logits``: ``[len(uids), vocab]`` from their prefills."""
+               stop: Optional[Callable[[int, int], bool]] = None, controls: Optional[LogitControls] = None) -> List[List[int]]:
+        """Batched decode of resident sessions. ``first_logits``: ``[len(uids), vocab]`` from their prefills. ``controls`` (of these sessions,
+        in this order; used up by the call): penalties, biases and masks on every step's logits."""
         out: List[List[int]] = [[] for _ in uids]
         logits = first_logits
         alive = list(range(len(uids)))
         for step in range(max_new_tokens):
-            nxt = sample_next(logits, do_sample, temperature, top_k, top_p).cpu()
-            keep = []
+            nxt = sample_next(logits, do_sample, temperature, top_k, top_p, controls).cpu()
+            keep, places = [], []
             for j, i in enumerate(alive):
                 tok = int(nxt[j])
                 out[i].append(tok)
                 if not (stop and stop(uids[i], tok)):
                     keep.append((i, tok))
+                    places.append(j)
             if not keep or step == max_new_tokens - 1:
                 break
+            if controls is not None:
+                controls.keep(places)
             alive = [i for i, _ in keep]
             toks = [torch.tensor([t], dtype=torch.int32) for _, t in keep]
             logits, lats = self.engine.put([uids[i] for i in alive], toks, capture_latents=True)

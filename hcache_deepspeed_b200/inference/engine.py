@@ -414,8 +414,10 @@ class InferenceEngine(torch.nn.Module):
     # ---- generation ----------------------------------------------------------------------------------------
     @torch.no_grad()
     def generate(self, *inputs, **kwargs):
-        """Injected: greedy / temperature / top-k / top-p sampling over sessions. Otherwise HF ``generate``
-        (``num_beams > 1`` is rejected exactly as in the reference, engine.py:583-606)."""
+        """Injected: greedy / temperature / top-k / top-p sampling over sessions, under ``repetition_penalty``, ``presence_penalty``,
+        ``frequency_penalty`` (numbers, or lists with one per row), ``logit_bias`` (a dict, or a list of them) and ``allowed`` (bool
+        ``[rows, vocab]``), see :class:`LogitControls`. Otherwise HF ``generate`` (``num_beams > 1`` is rejected exactly as in the reference,
+        engine.py:583-606)."""
         num_beams = kwargs.get("num_beams", 1)
         gc = kwargs.get("generation_config", None)
         if gc is not None:
@@ -444,21 +446,29 @@ class InferenceEngine(torch.nn.Module):
         if ephemeral:
             session_ids = [self._next_ephemeral_uid + i for i in range(Bsz)]
             self._next_ephemeral_uid += Bsz
-        from .sampling import sample_next
-        out = self._injected_forward(ids, session_ids=session_ids, last_token_only=True,
-                                     attention_mask=kwargs.get("attention_mask"))
+        from .sampling import LogitControls, sample_next
+        attention_mask = kwargs.get("attention_mask")
+        out = self._injected_forward(ids, session_ids=session_ids, last_token_only=True, attention_mask=attention_mask)
         seqs = [ids[b].tolist() for b in range(Bsz)]
+        wanted = {k: kwargs[k] for k in ("repetition_penalty", "presence_penalty", "frequency_penalty", "logit_bias", "allowed") if kwargs.get(k) is not None}
+        controls = None
+        if wanted:
+            told = [ids[b] if attention_mask is None else ids[b][attention_mask[b].bool()] for b in range(Bsz)]
+            controls = LogitControls(told, out.logits.shape[-1], max_new, out.logits.device, **wanted)
         alive = list(range(Bsz))
         for step in range(max_new):
-            nxt = sample_next(out.logits, do_sample, temperature, top_k, top_p).cpu()
-            still = []
+            nxt = sample_next(out.logits, do_sample, temperature, top_k, top_p, controls).cpu()
+            still, places = [], []
             for j, b in enumerate(alive):
                 tok = int(nxt[j])
                 seqs[b].append(tok)
                 if tok not in eos_set:
                     still.append((b, tok))
+                    places.append(j)
             if not still or step == max_new - 1:
                 break
+            if controls is not None:
+                controls.keep(places)
             alive = [b for b, _ in still]
             step_ids = torch.tensor([[t] for _, t in still])
             out = self._injected_forward(step_ids, session_ids=[session_ids[b] for b in alive], last_token_only=True)

@@ -175,3 +175,18 @@ class BlockedFlashAttn(DSKernelBase):
             self._ops(q).attention(q, out, kv_cache_layer, batch, n_q, n_kv, self.d, self.scale)
             return out
         return ref.paged_attention(q, kv_cache_layer, block_tables, items, n_q, n_kv, self.scale, out=out)
+
+
+class SharedPrefixAttn(DSKernelBase):
+    """Causal attention of a batch whose sequences share prefixes, against the paged KV cache: each prefix is read once for its group
+    (``ops.plans.SharedPrefixPlan`` says which sequences share what). 16-bit, head sizes 64 and 128 on a GPU."""
+
+    def __init__(self, head_size: int, dtype: torch.dtype, scale: Optional[float] = None):
+        self._check_dtype(dtype)
+        self.d = head_size
+        self.scale = scale if scale is not None else ref.attention_scale(head_size)
+
+    def __call__(self, out, q, kv_cache_layer, block_tables, plan):
+        if plan.head_dim != self.d:
+            raise ValueError(f"the plan is for heads of {plan.head_dim} values, this attention has {self.d}")
+        return self._ops(q).attention_shared(q, out, kv_cache_layer, block_tables, plan, self.scale)

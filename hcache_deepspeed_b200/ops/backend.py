@@ -258,6 +258,29 @@ class CpuOps:
         return self.routed_experts(x, ids, lw, f, act, shared, out, bufs)
 
     # ---- misc ---------------------------------------------------------------------------------------
+    # ---- batches of many requests ---------------------------------------------------------------------
+    def adapter_add(self, base, x, down, up, scales, plan, out):
+        if plan.n_rows != x.shape[0] or plan.n_adapters != down.shape[0]:
+            raise ValueError(f"the plan is for {plan.n_rows} rows of {plan.n_adapters} adapters, the call has {x.shape[0]} of {down.shape[0]}")
+        out.copy_(ref.adapter_add(base, x, down, up, scales, plan.ids))
+        return out
+
+    def attention_shared(self, q, out, kv_layer, block_tables, plan, scale):
+        T, d = plan.rows, plan.head_dim
+        items = torch.tensor([(i, r, n, k - n) for (i, r, n, k) in plan.items[:, :4].tolist() if n], dtype=torch.int32)
+        if T:
+            q3, o3 = q[:T].reshape(T, plan.n_q_heads, d), torch.empty(T, plan.n_q_heads, d, dtype=out.dtype)
+            ref.paged_attention(q3, kv_layer, block_tables, items, plan.n_q_heads, plan.n_kv_heads, scale, out=o3)
+            out[:T] = o3.reshape(T, -1)
+        return out
+
+    def logit_controls(self, logits, out, **controls):
+        from .kernels import _check_controls
+        names = ("history", "history_len", "prompt_len", "repetition", "presence", "frequency", "bias_ids", "bias", "mask", "mask_rows")
+        _check_controls(logits, out, *(controls.get(n) for n in names))
+        out.copy_(ref.logit_controls(logits, **controls))
+        return out
+
     def embed(self, ids, weight, out, pos_weight=None, tok_pos=None, pos_offset=0):
         out.copy_(ref.embed(ids, weight, pos_weight, tok_pos, pos_offset))
         return out
@@ -573,6 +596,15 @@ class CudaOps:
     def delta_rule(self, proj, lw, m, state, conv_state, spans, n_single, conv_buf, dt_buf, y, out, eps, workspace):
         return self.k.delta_rule(proj, lw.ssm_conv_w, lw.ssm_conv_b, lw.ssm_dt_bias, lw.ssm_a, state, conv_state, spans, n_single, m.groups,
                                  conv_buf, dt_buf, y, out, lw.ssm_norm, eps, workspace)
+
+    def adapter_add(self, base, x, down, up, scales, plan, out):
+        return self.k.adapter_add(base, x, down, up, scales, plan, out=out)
+
+    def attention_shared(self, q, out, kv_layer, block_tables, plan, scale):
+        return self.k.paged_attention_shared(q, out, kv_layer, block_tables, plan, scale)
+
+    def logit_controls(self, logits, out, **controls):
+        return self.k.logit_controls(logits, out, **controls)
 
     def embed(self, ids, weight, out, pos_weight=None, tok_pos=None, pos_offset=0):
         return self.k.embed(ids, weight, out, pos_weight=pos_weight, tok_pos=tok_pos, pos_offset=pos_offset)

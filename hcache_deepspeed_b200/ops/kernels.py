@@ -17,6 +17,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import native
+from .plans import AdapterPlan, SharedPrefixPlan  # noqa: F401
 
 ACT_IDENTITY, ACT_GELU, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_SWIGLU_CLAMPED, ACT_RELU2 = 0, 1, 2, 3, 4, 5, 6
 ACT_CODES = {"identity": 0, None: 0, "gelu": 1, "relu": 2, "silu": 3, "gelu_tanh": 4, "gelu_new": 4,
@@ -964,3 +965,176 @@ def retention_stuck() -> bool:
     flag = ctypes.c_int(0)
     native.check(native.cuda_lib().hds_retention_status(ctypes.addressof(flag)), "hds_retention_status")
     return bool(flag.value)
+
+
+# ------------------------------------------------------------------------------------------------
+# batches of many requests: adapters beside a projection, attention behind a shared prefix, controls on logits
+# ------------------------------------------------------------------------------------------------
+def _same_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the call is on {device}")
+
+
+def _require_cuda(t: torch.Tensor, name: str) -> torch.device:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.device
+
+
+def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[t] = base[t] + scales[i] * (x[t] @ down[i].T) @ up[i].T`` with row t's own adapter ``i`` (``plan``), ``out[t] = base[t]`` for a row
+    without one. ``base`` [T, N] (the shared projection's output), ``x`` [T, K], ``down`` [adapters, R, K], ``up`` [adapters, N, R], 16-bit;
+    ``scales`` fp32 [adapters]. K, N and R are multiples of 8, R at most 256. ``out`` may be ``base``."""
+    device = _require_cuda(x, "x")
+    _check_2d(x, "x")
+    _check_2d(base, "base")
+    dt = _dt(x)
+    T, K = x.shape
+    N = base.shape[1]
+    if down.dim() != 3 or up.dim() != 3 or not down.is_contiguous() or not up.is_contiguous():
+        raise ValueError("down and up must be contiguous [adapters, rank, K] and [adapters, N, rank]")
+    n, R = down.shape[0], down.shape[1]
+    if base.shape[0] != T or down.shape[2] != K or tuple(up.shape) != (n, N, R) or scales.shape != (n, ):
+        raise ValueError(f"shapes do not agree: base {tuple(base.shape)}, x {tuple(x.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)}, "
+                         f"scales {tuple(scales.shape)}")
+    if not (base.dtype == down.dtype == up.dtype == x.dtype) or scales.dtype != torch.float32 or not scales.is_contiguous():
+        raise TypeError("base, x, down and up have one type, scales are contiguous fp32")
+    if R % 8 or not 8 <= R <= 256 or K % 8 or N % 8 or not K or not N:
+        raise ValueError(f"K, N and the rank are multiples of 8, the rank at most 256; got {K}, {N}, {R}")
+    if plan.n_rows != T or plan.n_adapters != n:
+        raise ValueError(f"the plan is for {plan.n_rows} rows of {plan.n_adapters} adapters, the call has {T} of {n}")
+    if out is None:
+        out = torch.empty((T, N), dtype=x.dtype, device=device)
+    _check_2d(out, "out")
+    if out.shape != base.shape or out.dtype != x.dtype:
+        raise ValueError("out must be like base")
+    _same_device(device, base=base, down=down, up=up, scales=scales, out=out)
+    if plan._dev is None or plan._dev.device != device:
+        raise ValueError(f"the plan is on {plan.device}, the call is on {device}")
+    in_place = out.data_ptr() == base.data_ptr() and out.stride(0) == base.stride(0)
+    lib = native.cuda_lib()
+    with torch.cuda.device(device):
+        for rows, tiles, count in plan.launches(copy_bare=not in_place):
+            rc = lib.hds_adapter_add(_p(base), base.stride(0), _p(x), x.stride(0), _p(down), _p(up), _p(scales), n, R, K, N, _p(plan.order), tiles,
+                                     count, rows, _p(out), out.stride(0), dt, _stream())
+            native.check(rc, "hds_adapter_add")
+            _count()
+    return out
+
+
+def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: torch.Tensor, block_tables: torch.Tensor, plan: SharedPrefixPlan,
+                           scale: float) -> torch.Tensor:
+    """Causal attention of a batch whose sequences share prefixes (``plan``), each prefix read once for its group. ``q`` and ``out``
+    [rows, n_q_heads * head_dim], a sequence's new tokens being neighbouring rows in the plan's order; rows behind the last sequence are left as they
+    are. ``kv_cache_layer`` [blocks, 2, n_kv_heads, block_size, head_dim] holds the new tokens' keys already; ``block_tables`` int32
+    [sequences, stride]. head_dim 64 or 128, 16-bit. A group's pages are those that its first sequence's table names."""
+    device = _require_cuda(q, "q")
+    _check_2d(q, "q")
+    _check_2d(out, "out")
+    dt = _dt(q)
+    d = plan.head_dim
+    if d not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {d}")
+    if q.shape[1] != plan.n_q_heads * d or q.shape[0] < plan.rows or out.shape[1] != q.shape[1] or out.shape[0] < plan.rows:
+        raise ValueError(f"q and out need {plan.rows} rows of {plan.n_q_heads} x {d}, got {tuple(q.shape)} and {tuple(out.shape)}")
+    if out.dtype != q.dtype or kv_cache_layer.dtype != q.dtype:
+        raise TypeError("q, out and the cache have one type")
+    if kv_cache_layer.dim() != 5 or tuple(kv_cache_layer.shape[1:]) != (2, plan.n_kv_heads, plan.block_size, d) or not kv_cache_layer.is_contiguous():
+        raise ValueError(f"the cache must be contiguous [blocks, 2, {plan.n_kv_heads}, {plan.block_size}, {d}], got {tuple(kv_cache_layer.shape)}")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1 or block_tables.shape[0] < plan.n_seqs or \
+            block_tables.shape[1] < plan.max_blocks:
+        raise ValueError(f"block_tables must be int32 [{plan.n_seqs}, at least {plan.max_blocks}], got {tuple(block_tables.shape)}")
+    _same_device(device, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
+    if plan._dev is None or plan._dev.device != device:
+        raise ValueError(f"the plan is on {plan.device}, the call is on {device}")
+    if plan.rows == 0:
+        return out
+    lib = native.cuda_lib()
+    tiles, items = plan.pointers()
+    with torch.cuda.device(device):
+        ws, n_bytes = None, 0
+        if plan.n_tiles:      # of this call alone: a plan may be in use on several streams, and in graphs
+            n_bytes = int(lib.hds_paged_attention_shared_workspace_bytes(plan.rows, plan.n_q_heads, d, plan.p_splits))
+            ws = torch.empty(n_bytes, dtype=torch.uint8, device=device)
+        rc = lib.hds_paged_attention_shared(_p(q), q.stride(0), _p(out), out.stride(0), plan.rows, _p(kv_cache_layer), kv_cache_layer.shape[0],
+                                            _p(block_tables), block_tables.stride(0), tiles, plan.n_tiles, plan.p_splits, items, plan.n_seqs,
+                                            plan.max_tokens, plan.o_splits, plan.n_q_heads, plan.n_kv_heads, d, plan.block_size, scale, _p(ws), n_bytes,
+                                            dt, _stream())
+    native.check(rc, "hds_paged_attention_shared")
+    _count(2 if plan.n_tiles else 1)
+    return out
+
+
+def _check_controls(logits: torch.Tensor, out: torch.Tensor, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask,
+                    mask_rows) -> None:
+    """What :func:`logit_controls` takes; the restatement in torch has the same checks."""
+    _check_2d(logits, "logits")
+    _check_2d(out, "out")
+    n, V = logits.shape
+    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"unsupported logits dtype {logits.dtype}: bf16, fp16 or fp32")
+    if out.shape != logits.shape or out.dtype != logits.dtype:
+        raise ValueError("out must be like logits")
+    if n > 65535 or V >= 1 << 30:
+        raise ValueError("at most 65535 rows and a vocabulary below 2^30")
+    if (history is None) != (history_len is None):
+        raise ValueError("a history comes with its lengths")
+    if history is None and any(t is not None for t in (prompt_len, repetition, presence, frequency)):
+        raise ValueError("penalties need a history")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("biases come with their tokens")
+    if mask is None and mask_rows is not None:
+        raise ValueError("mask_rows needs masks")
+
+    def rows_2d(t, name, dtype, rows, cols=None):
+        if t.dim() != 2 or t.dtype != dtype or t.stride(1) != 1 and t.shape[1] > 1 or (rows is not None and t.shape[0] != rows) or \
+                (cols is not None and t.shape[1] < cols):
+            raise ValueError(f"{name} must be {dtype} [{'masks' if rows is None else rows}, {'' if cols is None else cols}] with contiguous rows, got "
+                             f"{t.dtype} {tuple(t.shape)}")
+
+    if history is not None:
+        rows_2d(history, "history", torch.int32, n)
+    if bias is not None:
+        rows_2d(bias_ids, "bias_ids", torch.int32, n)
+        rows_2d(bias, "bias", torch.float32, n)
+        if bias.shape != bias_ids.shape:
+            raise ValueError("bias and bias_ids have one shape")
+    if mask is not None:
+        rows_2d(mask, "mask", torch.int32, n if mask_rows is None else None, -(-V // 32))
+    for name, t, dtype in (("history_len", history_len, torch.int32), ("prompt_len", prompt_len, torch.int32), ("repetition", repetition, torch.float32),
+                           ("presence", presence, torch.float32), ("frequency", frequency, torch.float32), ("mask_rows", mask_rows, torch.int32)):
+        if t is not None and (t.shape != (n, ) or t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous {dtype} [{n}], got {t.dtype} {tuple(t.shape)}")
+    _same_device(logits.device, out=out, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition, presence=presence,
+                 frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, mask_rows=mask_rows)
+
+
+def logit_controls(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, history: Optional[torch.Tensor] = None,
+                   history_len: Optional[torch.Tensor] = None, prompt_len: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
+                   presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, mask_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What every row's request lays on its logits ``[n, vocab]``, in this order (``out`` may be ``logits``):
+
+    ``repetition`` fp32 [n]: logits of tokens in the row's history are divided by it where positive, multiplied where not; ``frequency`` and
+    ``presence`` fp32 [n]: taken off once per time that the token stands in the answer, and once if it does. ``history`` int32 [n, places] holds
+    a row's tokens, the first ``history_len[i]`` of them, and of these the first ``prompt_len[i]`` are its prompt (default: none). ``bias``
+    fp32 [n, k] is added to the logits of the tokens ``bias_ids`` int32 [n, k] (of a token given twice the last one counts). ``mask`` int32
+    [masks, words]: bit v % 32 of word v // 32 allows token v, the others get -inf; ``mask_rows`` int32 [n]: the row's mask, or -1 for none
+    (default: mask i for row i). Ids that are no tokens (-1 as padding) are passed over."""
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    device = _require_cuda(logits, "logits")
+    _check_controls(logits, out, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask, mask_rows)
+    n, V = logits.shape
+    ld = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
+    wide = lambda t: 0 if t is None else t.shape[1]  # noqa: E731
+    with torch.cuda.device(device):
+        rc = native.cuda_lib().hds_logit_controls(_p(logits), logits.stride(0), _p(out), out.stride(0), n, V, _p(history), ld(history), wide(history),
+                                                  _p(history_len), _p(prompt_len), _p(repetition), _p(presence), _p(frequency), _p(bias_ids),
+                                                  ld(bias_ids), _p(bias), ld(bias), wide(bias), _p(mask), ld(mask),
+                                                  0 if mask is None else mask.shape[0], _p(mask_rows), _dt3(logits), _stream())
+    native.check(rc, "hds_logit_controls")
+    _count(1 if n and V else 0)
+    return out

@@ -1,0 +1,147 @@
+"""What the host works out once per batch for the kernels that share work among its requests; every layer's calls take the same plan.
+
+A plan belongs to one batch. Its arrays are on the device when the constructor returns, and no call changes them: calls on any stream, and
+captured graphs, may share one."""
+from __future__ import annotations
+
+from typing import Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+
+#: rows of a small and of a large tile of the adapter kernel
+ADAPTER_SMALL, ADAPTER_LARGE = 16, 64
+#: rows of one adapter that still go as small tiles
+ADAPTER_FEW = 32
+
+
+def _host_ints(values, name: str) -> np.ndarray:
+    if torch.is_tensor(values):
+        values = values.detach().cpu().numpy()
+    a = np.asarray(values if len(values) else np.zeros(0, dtype=np.int64))
+    if a.ndim != 1 or a.dtype.kind not in "iu":
+        raise ValueError(f"{name} must be a list of whole numbers")
+    return a.astype(np.int64)
+
+
+class AdapterPlan:
+    """Which rows go through which adapter. ``ids[t]``: the adapter of row t, negative for none. ``device``: where the calls run (host
+    memory: only the restatement in torch does)."""
+
+    def __init__(self, ids, n_adapters: int, device=None) -> None:
+        a = _host_ints(ids, "ids")
+        if a.size and int(a.max()) >= n_adapters:
+            raise ValueError(f"row {int(a.argmax())} has adapter {int(a.max())}, there are {n_adapters}")
+        if a.size >= 1 << 26:
+            raise ValueError("at most 2^26 rows")
+        self.ids, self.n_adapters, self.n_rows = np.where(a < 0, -1, a).astype(np.int32), int(n_adapters), int(a.size)
+        #: rows sorted by adapter, those without one first
+        order = np.argsort(self.ids, kind="stable").astype(np.int32)
+        names, starts, counts = np.unique(self.ids[order], return_index=True, return_counts=True)
+        tiles = {ADAPTER_SMALL: [], ADAPTER_LARGE: []}
+        self._bare_tiles = 0
+        for name, start, count in zip(names.tolist(), starts.tolist(), counts.tolist()):
+            if name < 0:
+                continue
+            stop = start + count
+            while start < stop:
+                left = stop - start
+                rows = ADAPTER_SMALL if left <= ADAPTER_FEW else ADAPTER_LARGE
+                tiles[rows].append((name, start, min(rows, left), 0))
+                start += rows
+        n_bare = int((self.ids < 0).sum())
+        #: tiles of rows without an adapter (they are copied, whatever the tile's size), behind the others of one of the two lists
+        bare = [(-1, i, min(ADAPTER_LARGE, n_bare - i), 0) for i in range(0, n_bare, ADAPTER_LARGE)]
+        host = ADAPTER_LARGE if tiles[ADAPTER_LARGE] else ADAPTER_SMALL
+        self._parts = [(rows, tiles[rows] + (bare if rows == host else []), len(bare) if rows == host else 0) for rows in (ADAPTER_LARGE, ADAPTER_SMALL)]
+        self.device = None if device is None else torch.device(device)
+        self._dev = None
+        if self.device is not None and self.device.type == "cuda":
+            pad = -order.size % 4        # tiles start on 16-byte boundaries
+            flat = [order, np.zeros(pad, dtype=np.int32)] + [np.asarray(t, dtype=np.int32).reshape(-1) for _, t, _ in self._parts]
+            self._dev = torch.from_numpy(np.concatenate(flat)).to(self.device)
+            self.order = self._dev[:order.size]
+            self._tiles_at = order.size + pad
+
+    def launches(self, copy_bare: bool):
+        """(tile rows, device pointer of the tiles, their number) of every launch; ``copy_bare``: rows without an adapter are written too."""
+        at = self._dev.data_ptr() + 4 * self._tiles_at
+        for rows, tiles, n_bare in self._parts:
+            n = len(tiles) - (0 if copy_bare else n_bare)
+            if n:
+                yield rows, at, n
+            at += 16 * len(tiles)
+
+
+class SharedPrefixPlan:
+    """A batch whose sequences share prefixes. ``new_tokens[i]`` query rows of sequence i (in this order in ``q``), behind ``keys[i]`` -
+    ``new_tokens[i]`` earlier tokens; ``groups``: (first sequence, sequences, prefix) - the block tables of these neighbouring sequences
+    begin with the same pages, for ``prefix`` tokens (a multiple of the block size, and none of the new ones). Sequences in no group share nothing."""
+
+    def __init__(self, new_tokens, keys, groups: Sequence[Tuple[int, int, int]], n_q_heads: int, n_kv_heads: int, head_dim: int, block_size: int,
+                 device=None) -> None:
+        new, kv = _host_ints(new_tokens, "new_tokens"), _host_ints(keys, "keys")
+        if new.shape != kv.shape:
+            raise ValueError("new_tokens and keys are lists of the same sequences")
+        if n_kv_heads < 1 or n_q_heads < 1 or n_q_heads % n_kv_heads or n_q_heads // n_kv_heads > 128:
+            raise ValueError(f"{n_q_heads} query heads do not share {n_kv_heads} KV heads (up to 128 each)")
+        if block_size not in (16, 32, 64, 128):
+            raise ValueError("block_size must be 16, 32, 64 or 128")
+        if (new < 0).any() or (new > kv).any() or kv.size and int(kv.max()) >= 1 << 31:
+            raise ValueError("a sequence has at least its new tokens as keys, and fewer than 2^31")
+        self.n_q_heads, self.n_kv_heads, self.head_dim, self.block_size = n_q_heads, n_kv_heads, head_dim, block_size
+        self.new_tokens, self.keys, self.groups = new, kv, [tuple(map(int, g)) for g in groups]
+        self.n_seqs, self.rows = int(new.size), int(new.sum())
+        if self.rows >= 1 << 24 or self.n_seqs > 65535:
+            raise ValueError("at most 65535 sequences with 2^24 new tokens in all")
+        prefix = np.zeros(new.size, dtype=np.int64)
+        row0 = np.concatenate([[0], np.cumsum(new)])
+        taken = np.zeros(new.size, dtype=bool)
+        tile_tokens, tiles = 128 // (n_q_heads // n_kv_heads), []
+        for first, n, length in self.groups:
+            if first < 0 or n < 1 or first + n > self.n_seqs or taken[first:first + n].any():
+                raise ValueError(f"group ({first}, {n}, {length}): sequences that are there, and in no other group")
+            if length < 0 or length % block_size or (length > kv[first:first + n] - new[first:first + n]).any():
+                raise ValueError(f"group ({first}, {n}, {length}): a prefix is whole pages ahead of the new tokens of all its sequences")
+            taken[first:first + n] = True
+            prefix[first:first + n] = length
+            if length:
+                lo, hi = int(row0[first]), int(row0[first + n])
+                tiles += [(first, r, min(tile_tokens, hi - r), length) for r in range(lo, hi, tile_tokens)]
+        self.prefix = prefix
+        self.max_tokens = int(new.max()) if new.size else 0
+        #: pages that the longest sequence needs in its block table
+        self.max_blocks = -(-int(kv.max()) // block_size) if kv.size else 0
+        live = new > 0
+        row_tiles = max(1, -(-self.max_tokens * (n_q_heads // n_kv_heads) // 8))
+        self.p_splits = pick_prefix_splits(len(tiles) * n_kv_heads, max((t[3] for t in tiles), default=0))
+        self.o_splits = pick_own_splits(int(live.sum()) * n_kv_heads * row_tiles, int((kv - prefix)[live].max()) if live.any() else 0)
+        self.n_tiles = len(tiles)
+        items = np.zeros((new.size, 8), dtype=np.int32)
+        items[:, 0], items[:, 1], items[:, 2], items[:, 3], items[:, 4] = np.arange(new.size), row0[:-1], new, kv, prefix
+        self.items = items
+        self.device = None if device is None else torch.device(device)
+        self._dev = None
+        if self.device is not None and self.device.type == "cuda":
+            host = np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), items.reshape(-1)])
+            self._dev = torch.from_numpy(host).to(self.device)
+
+    def pointers(self):
+        """Device pointers of the prefix' work list and of the sequences'."""
+        return self._dev.data_ptr(), self._dev.data_ptr() + 16 * self.n_tiles
+
+
+def pick_prefix_splits(units: int, prefix: int, sms: int = 148) -> int:
+    """Parts of a prefix of that many tokens, ``units`` CTAs wide: the fewest waves of SMs, a CTA's beginning and end counted as a tile and a half."""
+    tiles = -(-prefix // 128)
+    if units == 0 or tiles == 0:
+        return 1
+    return min(range(1, min(64, tiles) + 1), key=lambda s: (-(-units * s // sms) * (-(-tiles // s) + 1.5), s))
+
+
+def pick_own_splits(units: int, keys: int, sms: int = 148) -> int:
+    """CTAs in a cluster for a sequence's own keys: two CTAs per SM, as long as each has 128 keys (two strips per warp)."""
+    splits = 1
+    while splits < 8 and units * splits * 2 <= 2 * sms and keys >= 256 * splits:
+        splits *= 2
+    return splits

@@ -371,3 +371,55 @@ def retention_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log2_decay
         state.mul_(decay).add_(v[t].float()[:, :, None] * k[t][:, None, :])
         y[t] = (state * q[t].float()[:, None, :]).sum(-1)
     return y
+
+
+# ---- batches of many requests ------------------------------------------------------------------------------------------
+def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor, ids) -> torch.Tensor:
+    """``base[t] + scales[i] * (x[t] @ down[i].T) @ up[i].T`` with ``i = ids[t]``, or ``base[t]`` where it is negative."""
+    y = base.float()
+    if y is base:
+        y = base.clone()
+    ids = torch.as_tensor(ids).to(x.device).long()
+    for i in ids.unique().tolist():
+        if i >= 0:
+            rows = (ids == i).nonzero()[:, 0]
+            y[rows] += scales[i].float() * (x[rows].float() @ down[i].float().t() @ up[i].float().t())
+    return y.to(base.dtype)
+
+
+def logit_controls(logits: torch.Tensor, history=None, history_len=None, prompt_len=None, repetition=None, presence=None, frequency=None, bias_ids=None,
+                   bias=None, mask=None, mask_rows=None) -> torch.Tensor:
+    """Penalties, biases and masks on logits (``kernels.logit_controls``)."""
+    x = logits.float()
+    if x is logits:
+        x = logits.clone()
+    n, V = x.shape
+    if history is not None and history.shape[1]:
+        place = torch.arange(history.shape[1], device=x.device)[None]
+        live = (place < history_len[:, None]) & (history >= 0) & (history < V)
+        answer = live if prompt_len is None else live & (place >= prompt_len[:, None])
+        ids = history.long().clamp(0, V - 1) if V else history.long()
+        seen = torch.zeros(n, V, dtype=torch.int32, device=x.device).scatter_add_(1, ids, live.int()) > 0
+        count = torch.zeros(n, V, dtype=torch.int32, device=x.device).scatter_add_(1, ids, answer.int())
+        if repetition is not None:
+            r = repetition[:, None]
+            x = torch.where(seen, torch.where(x > 0, x / r, x * r), x)
+        if frequency is not None:
+            x = torch.where(count > 0, x - frequency[:, None] * count, x)
+        if presence is not None:
+            x = torch.where(count > 0, x - presence[:, None], x)
+    if bias is not None:
+        k = bias.shape[1]
+        good = (bias_ids >= 0) & (bias_ids < V)
+        last = torch.full((n, V), -1, dtype=torch.int64, device=x.device)       # of a token given twice the last one counts
+        last.scatter_reduce_(1, bias_ids.long().clamp(0, max(V - 1, 0)), torch.where(good, torch.arange(k, device=x.device)[None].expand(n, k), -1), "amax")
+        if k:
+            x = torch.where(last >= 0, x + bias.gather(1, last.clamp(min=0)), x)
+    if mask is not None and n and V:
+        token = torch.arange(V, device=x.device)
+        rows = torch.arange(n, device=x.device) if mask_rows is None else mask_rows.long()
+        ruled = (rows >= 0) & (rows < mask.shape[0])
+        if mask.shape[0]:
+            allowed = (mask[torch.where(ruled, rows, 0)][:, token // 32] >> (token % 32).to(torch.int32)) & 1
+            x = x.masked_fill((allowed == 0) & ruled[:, None], -math.inf)
+    return x.to(logits.dtype)

@@ -530,6 +530,38 @@ int64_t hds_retention_workspace_bytes(int T, int n_seqs, int heads, int vdim, in
 /* *stuck = 1 when a wait inside one of its kernels ever ran out of time (their results are then wrong). Synchronizes. */
 int hds_retention_status(int* stuck);
 
+/* ---- batches of many requests ---------------------------------------------------------------------------------------- */
+
+/* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scales[i] * (x[t] down[i]^T) up[i]^T. down
+ * [n_adapters][rank][width], up [n_adapters][outputs][rank], 16-bit (dtype 0 bf16, 1 fp16); scales fp32; rank, width and outputs multiples of 8,
+ * rank <= 256. order: rows sorted by adapter; tiles int32 [n_tiles][4] = (adapter, first place in order, rows <= tile_rows, 0), an adapter of
+ * -1 copying base (any number of rows). tile_rows 16 or 64. out may be base. All rows on 16-byte boundaries. */
+int hds_adapter_add(const void* base, int64_t ld_base, const void* x, int64_t ld_x, const void* down, const void* up, const float* scales,
+                    int n_adapters, int rank, int width, int outputs, const int32_t* order, const int32_t* tiles, int n_tiles, int tile_rows,
+                    void* out, int64_t ld_out, int dtype, void* stream);
+
+/* Paged attention of a batch whose sequences share prefixes. q and out: rows of n_q_heads * head_dim values, ld_q / ld_out apart; a group of
+ * neighbouring sequences reads its prefix once. tiles int32 [n_tiles][4] = (sequence whose table names the prefix' pages, first row, tokens <=
+ * 128 / (n_q_heads / n_kv_heads), prefix); items int32 [n_items][8] = (sequence, first row, new tokens, keys, prefix, 0, 0, 0): row t of them sees
+ * the keys up to keys - new tokens + t. Prefixes are whole pages ahead of the new tokens. p_splits (up to 64): parts of a prefix, o_splits
+ * (1 / 2 / 4 / 8): CTAs for a sequence's other keys. workspace: see below; nothing in it outlives the call. dtype 0 / 1. */
+int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out, int64_t ld_out, int rows, const void* kv_cache_layer, int64_t num_blocks,
+                               const int32_t* block_tables, int max_blocks_per_seq, const int32_t* tiles, int n_tiles, int p_splits,
+                               const int32_t* items, int n_items, int max_tokens, int o_splits, int n_q_heads, int n_kv_heads, int head_dim,
+                               int block_size, float scale, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+int64_t hds_paged_attention_shared_workspace_bytes(int rows, int n_q_heads, int head_dim, int p_splits);
+
+/* What requests lay on their logits [rows, vocab] (dtype 0 / 1 / 2), out likewise (may be logits). Of history [rows, ld_history] the first
+ * min(history_len, capacity) tokens of a row count, the first prompt_len of them as its prompt: x = x > 0 ? x / repetition : x * repetition for
+ * tokens of the history, then x -= frequency * count + presence * (count > 0) by the count in the answer; x += bias of the tokens in bias_ids
+ * [rows, n_bias] (of a token given twice the last one); x = -inf where the bit of mask mask_rows[row] (NULL: row) is 0; rows whose mask is none
+ * of the n_masks are free. history, prompt_len, repetition, presence, frequency, bias_ids, mask, mask_rows may be NULL. */
+int hds_logit_controls(const void* logits, int64_t ld_logits, void* out, int64_t ld_out, int rows, int vocab, const int32_t* history,
+                       int64_t ld_history, int capacity, const int32_t* history_len, const int32_t* prompt_len, const float* repetition,
+                       const float* presence, const float* frequency, const int32_t* bias_ids, int64_t ld_bias_ids, const float* bias,
+                       int64_t ld_bias, int n_bias, const uint32_t* mask, int64_t ld_mask, int n_masks, const int32_t* mask_rows, int dtype,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif
