@@ -970,16 +970,45 @@ def retention_stuck() -> bool:
 # ------------------------------------------------------------------------------------------------
 # batches of many requests: adapters beside a projection, attention behind a shared prefix, controls on logits
 # ------------------------------------------------------------------------------------------------
-def _same_device(device: torch.device, **tensors: Optional[torch.Tensor]) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the call is on {device}")
+# (A step makes hundreds of these calls: their checks read each attribute once, and a stream is asked for by its number. A Stream object and
+# a device guard alone cost 5 us of the 22 that a call took; it takes 9 to 12 so.)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _require_cuda(t: torch.Tensor, name: str) -> torch.device:
+def _place(t: torch.Tensor, name: str) -> int:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    return t.device
+    return t.get_device()
+
+
+def _elsewhere(index: int, **tensors: Optional[torch.Tensor]) -> None:
+    """Name the tensor that is not on the call's device."""
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, the call is on cuda:{index}")
+
+
+class _On:
+    """The call's device as the current one, for as long as it is not anyway."""
+
+    def __init__(self, index: int) -> None:
+        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+    def __enter__(self) -> None:
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc) -> None:
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _rows(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows of a 2-D tensor whose last dimension is contiguous (of a single row: its width)."""
+    st, shape = t.stride(), t.shape
+    if len(st) != 2 or st[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name} must be 2-D with a contiguous last dimension, got {tuple(shape)} / {st}")
+    return st[0] if shape[0] > 1 else shape[1]
 
 
 def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan,
@@ -987,39 +1016,40 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
     """``out[t] = base[t] + scales[i] * (x[t] @ down[i].T) @ up[i].T`` with row t's own adapter ``i`` (``plan``), ``out[t] = base[t]`` for a row
     without one. ``base`` [T, N] (the shared projection's output), ``x`` [T, K], ``down`` [adapters, R, K], ``up`` [adapters, N, R], 16-bit;
     ``scales`` fp32 [adapters]. K, N and R are multiples of 8, R at most 256. ``out`` may be ``base``."""
-    device = _require_cuda(x, "x")
-    _check_2d(x, "x")
-    _check_2d(base, "base")
-    dt = _dt(x)
-    T, K = x.shape
-    N = base.shape[1]
+    index = _place(x, "x")
+    ld_x, ld_base, dt, dtype = _rows(x, "x"), _rows(base, "base"), _dt(x), x.dtype
+    (T, K), (rows, N) = x.shape, base.shape
     if down.dim() != 3 or up.dim() != 3 or not down.is_contiguous() or not up.is_contiguous():
         raise ValueError("down and up must be contiguous [adapters, rank, K] and [adapters, N, rank]")
-    n, R = down.shape[0], down.shape[1]
-    if base.shape[0] != T or down.shape[2] != K or tuple(up.shape) != (n, N, R) or scales.shape != (n, ):
+    n, R, width = down.shape
+    if rows != T or width != K or up.shape != (n, N, R) or scales.shape != (n, ):
         raise ValueError(f"shapes do not agree: base {tuple(base.shape)}, x {tuple(x.shape)}, down {tuple(down.shape)}, up {tuple(up.shape)}, "
                          f"scales {tuple(scales.shape)}")
-    if not (base.dtype == down.dtype == up.dtype == x.dtype) or scales.dtype != torch.float32 or not scales.is_contiguous():
+    if base.dtype != dtype or down.dtype != dtype or up.dtype != dtype or scales.dtype != torch.float32 or not scales.is_contiguous():
         raise TypeError("base, x, down and up have one type, scales are contiguous fp32")
     if R % 8 or not 8 <= R <= 256 or K % 8 or N % 8 or not K or not N:
         raise ValueError(f"K, N and the rank are multiples of 8, the rank at most 256; got {K}, {N}, {R}")
     if plan.n_rows != T or plan.n_adapters != n:
         raise ValueError(f"the plan is for {plan.n_rows} rows of {plan.n_adapters} adapters, the call has {T} of {n}")
     if out is None:
-        out = torch.empty((T, N), dtype=x.dtype, device=device)
-    _check_2d(out, "out")
-    if out.shape != base.shape or out.dtype != x.dtype:
-        raise ValueError("out must be like base")
-    _same_device(device, base=base, down=down, up=up, scales=scales, out=out)
-    if plan._dev is None or plan._dev.device != device:
-        raise ValueError(f"the plan is on {plan.device}, the call is on {device}")
-    in_place = out.data_ptr() == base.data_ptr() and out.stride(0) == base.stride(0)
-    lib = native.cuda_lib()
-    with torch.cuda.device(device):
-        for rows, tiles, count in plan.launches(copy_bare=not in_place):
-            rc = lib.hds_adapter_add(_p(base), base.stride(0), _p(x), x.stride(0), _p(down), _p(up), _p(scales), n, R, K, N, _p(plan.order), tiles,
-                                     count, rows, _p(out), out.stride(0), dt, _stream())
-            native.check(rc, "hds_adapter_add")
+        out, ld_out = x.new_empty((T, N)), N
+    else:
+        ld_out = _rows(out, "out")
+        if out.shape != (T, N) or out.dtype != dtype:
+            raise ValueError("out must be like base")
+    if not index == base.get_device() == down.get_device() == up.get_device() == scales.get_device() == out.get_device():
+        _elsewhere(index, base=base, down=down, up=up, scales=scales, out=out)
+    if plan.index != index:
+        raise ValueError(f"the plan is on {plan.device}, the call is on cuda:{index}")
+    p_base, p_out = base.data_ptr(), out.data_ptr()
+    fn = native.cuda_lib().hds_adapter_add
+    with _On(index):
+        stream = _raw_stream(index)
+        for height, tiles, count in plan.launches if p_out != p_base or ld_out != ld_base else plan.launches_in_place:
+            rc = fn(p_base, ld_base, x.data_ptr(), ld_x, down.data_ptr(), up.data_ptr(), scales.data_ptr(), n, R, K, N, plan.order_ptr, tiles, count, height,
+                    p_out, ld_out, dt, stream)
+            if rc:
+                native.check(rc, "hds_adapter_add")
             _count()
     return out
 
@@ -1030,85 +1060,96 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     [rows, n_q_heads * head_dim], a sequence's new tokens being neighbouring rows in the plan's order; rows behind the last sequence are left as they
     are. ``kv_cache_layer`` [blocks, 2, n_kv_heads, block_size, head_dim] holds the new tokens' keys already; ``block_tables`` int32
     [sequences, stride]. head_dim 64 or 128, 16-bit. A group's pages are those that its first sequence's table names."""
-    device = _require_cuda(q, "q")
-    _check_2d(q, "q")
-    _check_2d(out, "out")
-    dt = _dt(q)
-    d = plan.head_dim
+    index = _place(q, "q")
+    ld_q, ld_out, dt, dtype = _rows(q, "q"), _rows(out, "out"), _dt(q), q.dtype
+    d, H, rows = plan.head_dim, plan.n_q_heads, plan.rows
     if d not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {d}")
-    if q.shape[1] != plan.n_q_heads * d or q.shape[0] < plan.rows or out.shape[1] != q.shape[1] or out.shape[0] < plan.rows:
-        raise ValueError(f"q and out need {plan.rows} rows of {plan.n_q_heads} x {d}, got {tuple(q.shape)} and {tuple(out.shape)}")
-    if out.dtype != q.dtype or kv_cache_layer.dtype != q.dtype:
+    (q_rows, q_width), (out_rows, out_width) = q.shape, out.shape
+    if q_width != H * d or q_rows < rows or out_width != q_width or out_rows < rows:
+        raise ValueError(f"q and out need {rows} rows of {H} x {d}, got {tuple(q.shape)} and {tuple(out.shape)}")
+    if out.dtype != dtype or kv_cache_layer.dtype != dtype:
         raise TypeError("q, out and the cache have one type")
-    if kv_cache_layer.dim() != 5 or tuple(kv_cache_layer.shape[1:]) != (2, plan.n_kv_heads, plan.block_size, d) or not kv_cache_layer.is_contiguous():
+    blocks = kv_cache_layer.shape[0] if kv_cache_layer.dim() == 5 else 0
+    if kv_cache_layer.shape != (blocks, 2, plan.n_kv_heads, plan.block_size, d) or not kv_cache_layer.is_contiguous():
         raise ValueError(f"the cache must be contiguous [blocks, 2, {plan.n_kv_heads}, {plan.block_size}, {d}], got {tuple(kv_cache_layer.shape)}")
-    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or block_tables.stride(1) != 1 or block_tables.shape[0] < plan.n_seqs or \
-            block_tables.shape[1] < plan.max_blocks:
-        raise ValueError(f"block_tables must be int32 [{plan.n_seqs}, at least {plan.max_blocks}], got {tuple(block_tables.shape)}")
-    _same_device(device, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
-    if plan._dev is None or plan._dev.device != device:
-        raise ValueError(f"the plan is on {plan.device}, the call is on {device}")
-    if plan.rows == 0:
+    ld_tables = _rows(block_tables, "block_tables")
+    if block_tables.dtype != torch.int32 or block_tables.shape[0] < plan.n_seqs or block_tables.shape[1] < plan.max_blocks:
+        raise ValueError(f"block_tables must be int32 [{plan.n_seqs}, at least {plan.max_blocks}], got {block_tables.dtype} {tuple(block_tables.shape)}")
+    if not index == out.get_device() == kv_cache_layer.get_device() == block_tables.get_device():
+        _elsewhere(index, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
+    if plan.index != index:
+        raise ValueError(f"the plan is on {plan.device}, the call is on cuda:{index}")
+    if rows == 0:
         return out
     lib = native.cuda_lib()
-    tiles, items = plan.pointers()
-    with torch.cuda.device(device):
+    with _On(index):
         ws, n_bytes = None, 0
         if plan.n_tiles:      # of this call alone: a plan may be in use on several streams, and in graphs
-            n_bytes = int(lib.hds_paged_attention_shared_workspace_bytes(plan.rows, plan.n_q_heads, d, plan.p_splits))
-            ws = torch.empty(n_bytes, dtype=torch.uint8, device=device)
-        rc = lib.hds_paged_attention_shared(_p(q), q.stride(0), _p(out), out.stride(0), plan.rows, _p(kv_cache_layer), kv_cache_layer.shape[0],
-                                            _p(block_tables), block_tables.stride(0), tiles, plan.n_tiles, plan.p_splits, items, plan.n_seqs,
-                                            plan.max_tokens, plan.o_splits, plan.n_q_heads, plan.n_kv_heads, d, plan.block_size, scale, _p(ws), n_bytes,
-                                            dt, _stream())
-    native.check(rc, "hds_paged_attention_shared")
+            n_bytes = int(lib.hds_paged_attention_shared_workspace_bytes(rows, H, d, plan.p_splits))
+            ws = q.new_empty(n_bytes // q.element_size())
+        rc = lib.hds_paged_attention_shared(q.data_ptr(), ld_q, out.data_ptr(), ld_out, rows, kv_cache_layer.data_ptr(), blocks, block_tables.data_ptr(), ld_tables,
+                                            plan.tiles_ptr, plan.n_tiles, plan.p_splits, plan.items_ptr, plan.n_seqs, plan.max_tokens, plan.o_splits, H,
+                                            plan.n_kv_heads, d, plan.block_size, scale, _p(ws), n_bytes, dt, _raw_stream(index))
+    if rc:
+        native.check(rc, "hds_paged_attention_shared")
     _count(2 if plan.n_tiles else 1)
     return out
 
 
+def _check_rows(t: torch.Tensor, name: str, dtype: torch.dtype, rows: Optional[int], cols: int = 0) -> int:
+    ld = _rows(t, name)
+    shape = t.shape
+    if t.dtype != dtype or rows is not None and shape[0] != rows or shape[1] < cols:
+        raise ValueError(f"{name} must be {dtype} [{'masks' if rows is None else rows}, {f'at least {cols}' if cols else 'any'}], got {t.dtype} {tuple(shape)}")
+    return ld
+
+
+def _check_each(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, n: int) -> None:
+    if t is not None and (t.dtype != dtype or t.shape != (n, ) or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous {dtype} [{n}], got {t.dtype} {tuple(t.shape)}")
+
+
 def _check_controls(logits: torch.Tensor, out: torch.Tensor, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask,
-                    mask_rows) -> None:
-    """What :func:`logit_controls` takes; the restatement in torch has the same checks."""
-    _check_2d(logits, "logits")
-    _check_2d(out, "out")
-    n, V = logits.shape
-    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"unsupported logits dtype {logits.dtype}: bf16, fp16 or fp32")
-    if out.shape != logits.shape or out.dtype != logits.dtype:
+                    mask_rows) -> Tuple[int, ...]:
+    """What :func:`logit_controls` takes, and the restatement in torch: elements between the rows of logits, out, history, bias_ids, bias and mask."""
+    ld, ld_out, shape, dtype = _rows(logits, "logits"), _rows(out, "out"), logits.shape, logits.dtype
+    n, V = shape
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"unsupported logits dtype {dtype}: bf16, fp16 or fp32")
+    if out.shape != shape or out.dtype != dtype:
         raise ValueError("out must be like logits")
     if n > 65535 or V >= 1 << 30:
         raise ValueError("at most 65535 rows and a vocabulary below 2^30")
-    if (history is None) != (history_len is None):
+    ld_history = ld_ids = ld_bias = ld_mask = 0
+    if history is not None and history_len is not None:
+        ld_history = _check_rows(history, "history", torch.int32, n)
+        _check_each(history_len, "history_len", torch.int32, n)
+        _check_each(prompt_len, "prompt_len", torch.int32, n)
+        _check_each(repetition, "repetition", torch.float32, n)
+        _check_each(presence, "presence", torch.float32, n)
+        _check_each(frequency, "frequency", torch.float32, n)
+    elif history is not None or history_len is not None:
         raise ValueError("a history comes with its lengths")
-    if history is None and any(t is not None for t in (prompt_len, repetition, presence, frequency)):
+    elif prompt_len is not None or repetition is not None or presence is not None or frequency is not None:
         raise ValueError("penalties need a history")
-    if (bias_ids is None) != (bias is None):
-        raise ValueError("biases come with their tokens")
-    if mask is None and mask_rows is not None:
-        raise ValueError("mask_rows needs masks")
-
-    def rows_2d(t, name, dtype, rows, cols=None):
-        if t.dim() != 2 or t.dtype != dtype or t.stride(1) != 1 and t.shape[1] > 1 or (rows is not None and t.shape[0] != rows) or \
-                (cols is not None and t.shape[1] < cols):
-            raise ValueError(f"{name} must be {dtype} [{'masks' if rows is None else rows}, {'' if cols is None else cols}] with contiguous rows, got "
-                             f"{t.dtype} {tuple(t.shape)}")
-
-    if history is not None:
-        rows_2d(history, "history", torch.int32, n)
-    if bias is not None:
-        rows_2d(bias_ids, "bias_ids", torch.int32, n)
-        rows_2d(bias, "bias", torch.float32, n)
+    if bias is not None and bias_ids is not None:
+        ld_ids, ld_bias = _check_rows(bias_ids, "bias_ids", torch.int32, n), _check_rows(bias, "bias", torch.float32, n)
         if bias.shape != bias_ids.shape:
             raise ValueError("bias and bias_ids have one shape")
+    elif bias is not None or bias_ids is not None:
+        raise ValueError("biases come with their tokens")
     if mask is not None:
-        rows_2d(mask, "mask", torch.int32, n if mask_rows is None else None, -(-V // 32))
-    for name, t, dtype in (("history_len", history_len, torch.int32), ("prompt_len", prompt_len, torch.int32), ("repetition", repetition, torch.float32),
-                           ("presence", presence, torch.float32), ("frequency", frequency, torch.float32), ("mask_rows", mask_rows, torch.int32)):
-        if t is not None and (t.shape != (n, ) or t.dtype != dtype or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous {dtype} [{n}], got {t.dtype} {tuple(t.shape)}")
-    _same_device(logits.device, out=out, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition, presence=presence,
-                 frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, mask_rows=mask_rows)
+        ld_mask = _check_rows(mask, "mask", torch.int32, n if mask_rows is None else None, -(-V // 32))
+        _check_each(mask_rows, "mask_rows", torch.int32, n)
+    elif mask_rows is not None:
+        raise ValueError("mask_rows needs masks")
+    index = logits.get_device()
+    for t in (out, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask, mask_rows):
+        if t is not None and t.get_device() != index:
+            _elsewhere(index, out=out, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition, presence=presence,
+                       frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, mask_rows=mask_rows)
+    return ld, ld_out, ld_history, ld_ids, ld_bias, ld_mask
 
 
 def logit_controls(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, history: Optional[torch.Tensor] = None,
@@ -1123,18 +1164,19 @@ def logit_controls(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, 
     fp32 [n, k] is added to the logits of the tokens ``bias_ids`` int32 [n, k] (of a token given twice the last one counts). ``mask`` int32
     [masks, words]: bit v % 32 of word v // 32 allows token v, the others get -inf; ``mask_rows`` int32 [n]: the row's mask, or -1 for none
     (default: mask i for row i). Ids that are no tokens (-1 as padding) are passed over."""
+    index = _place(logits, "logits")
     if out is None:
-        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
-    device = _require_cuda(logits, "logits")
-    _check_controls(logits, out, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask, mask_rows)
+        out = logits.new_empty(logits.shape)
+    ld, ld_out, ld_history, ld_ids, ld_bias, ld_mask = _check_controls(logits, out, history, history_len, prompt_len, repetition, presence, frequency,
+                                                                       bias_ids, bias, mask, mask_rows)
     n, V = logits.shape
-    ld = lambda t: 0 if t is None else t.stride(0)  # noqa: E731
-    wide = lambda t: 0 if t is None else t.shape[1]  # noqa: E731
-    with torch.cuda.device(device):
-        rc = native.cuda_lib().hds_logit_controls(_p(logits), logits.stride(0), _p(out), out.stride(0), n, V, _p(history), ld(history), wide(history),
-                                                  _p(history_len), _p(prompt_len), _p(repetition), _p(presence), _p(frequency), _p(bias_ids),
-                                                  ld(bias_ids), _p(bias), ld(bias), wide(bias), _p(mask), ld(mask),
-                                                  0 if mask is None else mask.shape[0], _p(mask_rows), _dt3(logits), _stream())
-    native.check(rc, "hds_logit_controls")
+    with _On(index):
+        rc = native.cuda_lib().hds_logit_controls(logits.data_ptr(), ld, out.data_ptr(), ld_out, n, V, _p(history), ld_history,
+                                                  0 if history is None else history.shape[1], _p(history_len), _p(prompt_len), _p(repetition),
+                                                  _p(presence), _p(frequency), _p(bias_ids), ld_ids, _p(bias), ld_bias,
+                                                  0 if bias is None else bias.shape[1], _p(mask), ld_mask, 0 if mask is None else mask.shape[0],
+                                                  _p(mask_rows), _dt3(logits), _raw_stream(index))
+    if rc:
+        native.check(rc, "hds_logit_controls")
     _count(1 if n and V else 0)
     return out

@@ -4,7 +4,7 @@ A plan belongs to one batch. Its arrays are on the device when the constructor r
 captured graphs, may share one."""
 from __future__ import annotations
 
-from typing import Optional, Sequence, Tuple
+from typing import Sequence, Tuple
 
 import numpy as np
 import torch
@@ -39,7 +39,6 @@ class AdapterPlan:
         order = np.argsort(self.ids, kind="stable").astype(np.int32)
         names, starts, counts = np.unique(self.ids[order], return_index=True, return_counts=True)
         tiles = {ADAPTER_SMALL: [], ADAPTER_LARGE: []}
-        self._bare_tiles = 0
         for name, start, count in zip(names.tolist(), starts.tolist(), counts.tolist()):
             if name < 0:
                 continue
@@ -55,22 +54,20 @@ class AdapterPlan:
         host = ADAPTER_LARGE if tiles[ADAPTER_LARGE] else ADAPTER_SMALL
         self._parts = [(rows, tiles[rows] + (bare if rows == host else []), len(bare) if rows == host else 0) for rows in (ADAPTER_LARGE, ADAPTER_SMALL)]
         self.device = None if device is None else torch.device(device)
-        self._dev = None
+        #: device number (-1: not on a GPU); launches: (tile rows, device pointer of the tiles, their number), with and without the rows that are copied
+        self.index, self.launches, self.launches_in_place = -1, [], []
         if self.device is not None and self.device.type == "cuda":
             pad = -order.size % 4        # tiles start on 16-byte boundaries
             flat = [order, np.zeros(pad, dtype=np.int32)] + [np.asarray(t, dtype=np.int32).reshape(-1) for _, t, _ in self._parts]
             self._dev = torch.from_numpy(np.concatenate(flat)).to(self.device)
-            self.order = self._dev[:order.size]
-            self._tiles_at = order.size + pad
-
-    def launches(self, copy_bare: bool):
-        """(tile rows, device pointer of the tiles, their number) of every launch; ``copy_bare``: rows without an adapter are written too."""
-        at = self._dev.data_ptr() + 4 * self._tiles_at
-        for rows, tiles, n_bare in self._parts:
-            n = len(tiles) - (0 if copy_bare else n_bare)
-            if n:
-                yield rows, at, n
-            at += 16 * len(tiles)
+            self.index, self.order_ptr = self._dev.get_device(), self._dev.data_ptr()
+            at = self.order_ptr + 4 * (order.size + pad)
+            for rows, t, n_bare in self._parts:
+                if t:
+                    self.launches.append((rows, at, len(t)))
+                if len(t) > n_bare:
+                    self.launches_in_place.append((rows, at, len(t) - n_bare))
+                at += 16 * len(t)
 
 
 class SharedPrefixPlan:
@@ -121,14 +118,12 @@ class SharedPrefixPlan:
         items[:, 0], items[:, 1], items[:, 2], items[:, 3], items[:, 4] = np.arange(new.size), row0[:-1], new, kv, prefix
         self.items = items
         self.device = None if device is None else torch.device(device)
-        self._dev = None
+        #: device number (-1: not on a GPU) and device pointers of the prefix' work list and of the sequences'
+        self.index, self.tiles_ptr, self.items_ptr = -1, 0, 0
         if self.device is not None and self.device.type == "cuda":
-            host = np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), items.reshape(-1)])
-            self._dev = torch.from_numpy(host).to(self.device)
-
-    def pointers(self):
-        """Device pointers of the prefix' work list and of the sequences'."""
-        return self._dev.data_ptr(), self._dev.data_ptr() + 16 * self.n_tiles
+            self._dev = torch.from_numpy(np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), items.reshape(-1)])).to(self.device)
+            self.index, self.tiles_ptr = self._dev.get_device(), self._dev.data_ptr()
+            self.items_ptr = self.tiles_ptr + 16 * self.n_tiles
 
 
 def pick_prefix_splits(units: int, prefix: int, sms: int = 148) -> int:
