@@ -1,12 +1,15 @@
 // Low-rank adapters of many requests beside a shared projection:  out[t] = base[t] + scale[i] * (x[t] down[i]^T) up[i]^T,  i = ids[t].
 //
-// Rows are sorted by adapter (the plan's order), and a tile is up to 16 or 64 rows of one adapter. A cluster of 8 CTAs has a tile:
-//   1. h = x down^T: CTA r sums over its eighth of the width. Both operands go from memory to registers as mma.sync wants them (a sum
-//      does not mind its order, so a lane's 16 bytes of a row are two k-steps' worth).
-//   2. The eighths meet in shared memory, over the cluster: CTA r adds up the eighth r of the tile's h (in the order of the CTAs) and gives
-//      the sums to all of them. No scratch in global memory, no tickets: calls on several streams and captured graphs share nothing.
-//   3. out = base + scale h up^T: CTA r has an eighth of the outputs, in groups of 32 columns whose order in the MMA is such that a
-//      lane ends up with 8 neighbouring ones: base and out are moved 16 bytes at a time.
+// Rows are sorted by adapter (the plan's order), and a tile is up to 64 rows of one adapter. Both products run on mma.sync with operands that go
+// from memory to registers as the instruction wants them: a sum does not mind its order, so that a lane's 16 bytes of a row are two k-steps'
+// worth, and columns of the output are dealt out such that a lane ends up with 8 neighbouring ones, moved 16 bytes at a time.
+//
+// Few rows (a decode step, tiles of up to 16): one kernel. A cluster of 4 or 8 CTAs has a tile; each sums h = x down^T over its part of the
+// width, gives its sums to all of them, over the cluster, and has a part of the outputs. Nothing goes through memory, and what the second
+// product reads comes to shared memory while the first one runs.
+// Many rows: two kernels. The first sums h over a part of the width for a tile and leaves it in scratch, in fp32; the second has a tile and 256
+// outputs. It starts while the first one runs: its part of `up` and of `base` is in registers when h is there.
+//
 // h enters the second product as a 16-bit value and what its rounding left over, itself in 16 bits, so that it keeps 16 bits or more; fp16
 // rows are brought to a largest value of 2^8 ... 2^9 first (and back), since fp16 has no room for large h and few bits for small.
 //
@@ -18,22 +21,28 @@
 
 namespace hds {
 
-constexpr int kAdCluster = 8;
+constexpr int kAdCluster = 8;     // CTAs of a tile in the one kernel, at most
 constexpr int kAdThreads = 256;
 constexpr int kAdWarps = kAdThreads / 32;
 constexpr int kAdMaxRank = 256;
+constexpr int kAdRows = 64;       // of a tile
+constexpr int kAdFew = 16;        // of a tile that the one kernel takes
+constexpr int kAdCols = 256;      // outputs of a CTA of the second of two kernels
 
 struct AdapterArgs {
     const void* x;
     const void* base;
     void* out;
-    int64_t ld_x, ld_base, ld_out;
+    int ld_x, ld_base, ld_out;
     const void* down;       // [adapters][rank][width]
     const void* up;         // [adapters][outputs][rank]
     const float* scales;    // [adapters]
-    const int32_t* order;   // rows sorted by adapter
-    const int4* tiles;      // (adapter or -1, first place in order, rows, 0)
-    int n_adapters, rank, width, outputs;
+    const int4* tiles;      // (adapter or -1, place of the first row in the sorted order, rows, 0)
+    const int32_t* tile_rows;   // [tiles][64]: the rows, the last one repeated to the end
+    int n_adapters, rank, width, outputs, rows;
+    int cluster;            // CTAs of a tile: 4 or 8
+    int k_parts, k_part;    // parts of the width, and columns of each
+    float* h;               // [k_parts][rows][rank], by place in order
 };
 
 __device__ __forceinline__ uint32_t ad_cta_rank() {
@@ -41,242 +50,530 @@ __device__ __forceinline__ uint32_t ad_cta_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void ad_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void ad_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ad_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // the place of `p` in CTA `cta`'s shared memory
 __device__ __forceinline__ uint32_t ad_at(const void* p, uint32_t cta) {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(cta));
     return a;
 }
-__device__ __forceinline__ float4 ad_load4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ void ad_store4(uint32_t at, const float4& v) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 __device__ __forceinline__ uint4 ad_zero() { return make_uint4(0u, 0u, 0u, 0u); }
 
-template <int MT>
-__host__ __device__ constexpr int ad_rows() { return 16 * MT; }
 // h rows of 16-bit values: 8 more than the rank, so that the rows of a fragment lie in different banks
 __host__ __device__ constexpr int ad_pitch(int rank) { return (rank + 15) / 16 * 16 + 8; }
-// the warps' sums of a block of 64 of the rank, then those of the CTA and of all CTAs, then the two 16-bit parts of h
-template <int MT>
-__host__ __device__ constexpr size_t ad_smem_bytes(int rank) {
-    const int padded = (rank + 63) / 64 * 64;
-    return (static_cast<size_t>(kAdWarps) * 16 * 64 + ad_rows<MT>() * 64 + static_cast<size_t>(ad_rows<MT>()) * padded) * 4 +
-           static_cast<size_t>(2) * ad_rows<MT>() * ad_pitch(rank) * 2;
-}
 
-template <int MT, int NT, bool kBf16>
-__global__ void __launch_bounds__(kAdThreads) adapter_kernel(const AdapterArgs a) {
-    constexpr int M = ad_rows<MT>();
-    constexpr int KW = kAdWarps / MT;           // warps that share a tile of 16 rows
-    extern __shared__ __align__(16) uint8_t ad_smem[];
-    __shared__ float row_scale[M];
-    const int rank = a.rank, padded = (rank + 63) / 64 * 64, pitch = ad_pitch(rank);
-    float* red = reinterpret_cast<float*>(ad_smem);                   // [8 warps][16][64]
-    float* part = red + kAdWarps * 16 * 64;                           // [M][64]
-    float* h = part + M * 64;                                         // [M][padded]
-    uint16_t* h_hi = reinterpret_cast<uint16_t*>(h + M * padded);     // [M][pitch]
-    uint16_t* h_lo = h_hi + M * pitch;
-    pdl_enter();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t cta = ad_cta_rank();
-    const int4 tile = a.tiles[blockIdx.x / kAdCluster];
-    const int n_slice = (a.outputs + kAdCluster * 32 - 1) / (kAdCluster * 32) * 32;
-    const int n0 = static_cast<int>(cta) * n_slice, n1 = min(a.outputs, n0 + n_slice);
-    if (tile.x < 0 || tile.x >= a.n_adapters) {        // rows without an adapter (the whole cluster leaves here)
-        const int pieces = max(0, n1 - n0) / 8;
-        for (int i = tid; i < tile.z * pieces; i += kAdThreads) {
-            const int64_t row = a.order[tile.y + i / pieces];
-            const int64_t col = n0 + i % pieces * 8;
-            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row * a.ld_out + col) =
-                *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.base) + row * a.ld_base + col);
-        }
-        return;
-    }
-    const int mt = warp % MT, kw = warp / MT;
-    const int r0 = mt * 16 + g, r1 = r0 + 8;           // my two rows of the tile
-    const bool live0 = r0 < tile.z, live1 = r1 < tile.z;
-    const int64_t row0 = a.order[tile.y + (live0 ? r0 : 0)], row1 = a.order[tile.y + (live1 ? r1 : 0)];
-    const uint16_t* x0 = reinterpret_cast<const uint16_t*>(a.x) + row0 * a.ld_x;
-    const uint16_t* x1 = reinterpret_cast<const uint16_t*>(a.x) + row1 * a.ld_x;
+__device__ __forceinline__ const uint16_t* ad_row(const void* p, int row, int ld) { return reinterpret_cast<const uint16_t*>(p) + static_cast<int64_t>(row) * ld; }
 
-    // ---- 1. my eighth of the width, 32 columns at a time, shared out among the warps ----
-    const int k_slice = (a.width + kAdCluster * 32 - 1) / (kAdCluster * 32) * 32;
-    const int k0 = static_cast<int>(cta) * k_slice, k1 = min(a.width, k0 + k_slice);
-    const uint16_t* down = reinterpret_cast<const uint16_t*>(a.down) + static_cast<int64_t>(tile.x) * rank * a.width;
-    for (int rb = 0; rb < rank; rb += NT * 8) {
-        float acc[NT][4];
+// acc = 16 rows of x times NT * 8 rows of down (those from rb on), over the columns k0 to k1 in blocks of 32, of which this warp has number `b` and
+// every `step`-th after it. U of them are asked for at once: with fewer on the way the sum waits for memory (4099 rows x 4096, rank 32: 31.8 us
+// one by one). Rows of a tile that are not there repeat others, rows of down behind the rank the last ones: nobody looks at what they come to.
+// x1 may be x0.
+template <int NT, bool kBf16, int U>
+__device__ __forceinline__ void ad_down(float (&acc)[NT][4], const uint16_t* x0, const uint16_t* x1, const uint16_t* down, int rb, int rank, int width, int k0,
+                                        int k1, int b, int step, int g, int t) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-#pragma unroll 2
-        for (int k = k0 + kw * 32; k < k1; k += KW * 32) {
-            const int kk = k + t * 8;
-            const bool in = kk < k1;
-            const uint4 xa = in && live0 ? *reinterpret_cast<const uint4*>(x0 + kk) : ad_zero();
-            const uint4 xb = in && live1 ? *reinterpret_cast<const uint4*>(x1 + kk) : ad_zero();
-            uint4 d[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                d[j] = in && rb + j * 8 < rank ? ld_nc_v4(down + static_cast<int64_t>(rb + j * 8 + g) * a.width + kk) : ad_zero();
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                mma_m16n8k16<kBf16>(acc[j], xa.x, xb.x, xa.y, xb.y, d[j].x, d[j].y);
-                mma_m16n8k16<kBf16>(acc[j], xa.z, xb.z, xa.w, xb.w, d[j].z, d[j].w);
-            }
-        }
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
+    const int last = (rank - rb) / 8 - 1, whole = (k1 - k0) / 32;
+    const uint16_t* d0 = down + static_cast<int64_t>(rb + g) * width;
+    auto multiply = [&](const uint4& xa, const uint4& xb, const uint4 (&d)[NT]) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            *reinterpret_cast<float2*>(red + (warp * 16 + g) * 64 + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2*>(red + (warp * 16 + g + 8) * 64 + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+            mma_m16n8k16<kBf16>(acc[j], xa.x, xb.x, xa.y, xb.y, d[j].x, d[j].y);
+            mma_m16n8k16<kBf16>(acc[j], xa.z, xb.z, xa.w, xb.w, d[j].z, d[j].w);
         }
-        __syncthreads();
-        for (int i = tid; i < M * NT * 8; i += kAdThreads) {
-            const int r = i / (NT * 8), c = i % (NT * 8);
-            float s = 0.0f;
+    };
+    for (; b < whole; b += U * step) {
+        uint4 xa[U], xb[U], d[U][NT];
 #pragma unroll
-            for (int w = 0; w < KW; ++w) s += red[((w * MT + (r >> 4)) * 16 + (r & 15)) * 64 + c];
-            part[r * 64 + c] = s;
-        }
-        // ---- 2. the eighths of the width meet: CTA r adds up eighth r of this block of h ----
-        ad_cluster_sync();
-        constexpr int QUADS = M * NT * 8 / 4;
-        for (int i = tid; i < QUADS / kAdCluster; i += kAdThreads) {
-            const int q = static_cast<int>(cta) * (QUADS / kAdCluster) + i;
-            const int r = q / (NT * 2), c = q % (NT * 2) * 4;
-            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int u = 0; u < U; ++u)
+            if (b + u * step < whole) {
+                const int k = k0 + (b + u * step) * 32 + t * 8;
+                xa[u] = *reinterpret_cast<const uint4*>(x0 + k);
+                xb[u] = *reinterpret_cast<const uint4*>(x1 + k);
 #pragma unroll
-            for (int p = 0; p < kAdCluster; ++p) {
-                const float4 v = ad_load4(ad_at(part + r * 64 + c, p));
-                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+                for (int j = 0; j < NT; ++j) d[u][j] = *reinterpret_cast<const uint4*>(d0 + static_cast<int64_t>(min(j, last) * 8) * width + k);
             }
 #pragma unroll
-            for (int p = 0; p < kAdCluster; ++p) ad_store4(ad_at(h + r * padded + rb + c, p), s);
-        }
-        ad_cluster_sync();
+        for (int u = 0; u < U; ++u)
+            if (b + u * step < whole) multiply(xa[u], xb[u], d[u]);
     }
-    // ---- h in two 16-bit parts ----
+    // a last block of less than 32 columns is the turn of one warp
+    if ((k1 - k0) % 32 != 0 && (whole - b) % step == 0) {
+        const int k = k0 + whole * 32 + t * 8;
+        const bool in = k < k1;
+        uint4 d[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) d[j] = in ? *reinterpret_cast<const uint4*>(d0 + static_cast<int64_t>(min(j, last) * 8) * width + k) : ad_zero();
+        multiply(in ? *reinterpret_cast<const uint4*>(x0 + k) : ad_zero(), in ? *reinterpret_cast<const uint4*>(x1 + k) : ad_zero(), d);
+    }
+}
+
+// one row's largest |h| -> the power of two that brings it to 2^8 ... 2^9, and that power's reciprocal, both normal numbers
+__device__ __forceinline__ float2 ad_row_scale(float m) {
+    int e = 9;
+    if (m > 0.0f && m < INFINITY) frexpf(m, &e);
+    e = min(max(e - 9, -126), 126);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), __uint_as_float(static_cast<uint32_t>(127 + e) << 23));
+}
+template <bool kBf16>
+__device__ __forceinline__ void ad_split(float v, uint16_t& hi, uint16_t& lo) {
+    const uint32_t h = pack2<kBf16>(v, 0.0f);
+    const float rest = v - unpack_lo<kBf16>(h);
+    hi = static_cast<uint16_t>(h);
+    lo = static_cast<uint16_t>(pack2<kBf16>(fabsf(rest) < INFINITY ? rest : 0.0f, 0.0f));
+}
+
+// 16 rows (r0 and r0 + 8 are this lane's) by 32 outputs from n on. Tile j, column 2 t + e of the MMA is column 8 t + 2 j + e of the 32.
+template <bool kBf16>
+__device__ __forceinline__ void ad_up_step(float (&acc)[4][4], const uint16_t* h_hi, const uint16_t* h_lo, int pitch, int r0, int c, const uint2 (&u)[4]) {
+    const uint2 p0 = *reinterpret_cast<const uint2*>(h_hi + r0 * pitch + c), p1 = *reinterpret_cast<const uint2*>(h_hi + (r0 + 8) * pitch + c);
+    const uint2 l0 = *reinterpret_cast<const uint2*>(h_lo + r0 * pitch + c), l1 = *reinterpret_cast<const uint2*>(h_lo + (r0 + 8) * pitch + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        mma_m16n8k16<kBf16>(acc[j], p0.x, p1.x, p0.y, p1.y, u[j].x, u[j].y);
+        mma_m16n8k16<kBf16>(acc[j], l0.x, l1.x, l0.y, l1.y, u[j].x, u[j].y);
+    }
+}
+// this lane's values of four rows of `up` (2 j rows on from `up`, which points at its place of a k-step), of which `rows` are left; `in`: the k-step
+// has values for this lane
+__device__ __forceinline__ void ad_up_load(uint2 (&u)[4], const uint16_t* up, int rank, int rows, bool in) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = 2 * j < rows && in ? __ldg(reinterpret_cast<const uint2*>(up + 2 * j * rank)) : make_uint2(0u, 0u);
+}
+template <bool kBf16>
+__device__ __forceinline__ uint4 ad_join(const uint4& b, const float (&acc)[4][4], int e, float s) {
+    return make_uint4(pack2<kBf16>(fmaf(s, acc[0][e], unpack_lo<kBf16>(b.x)), fmaf(s, acc[0][e + 1], unpack_hi<kBf16>(b.x))),
+                      pack2<kBf16>(fmaf(s, acc[1][e], unpack_lo<kBf16>(b.y)), fmaf(s, acc[1][e + 1], unpack_hi<kBf16>(b.y))),
+                      pack2<kBf16>(fmaf(s, acc[2][e], unpack_lo<kBf16>(b.z)), fmaf(s, acc[2][e + 1], unpack_hi<kBf16>(b.z))),
+                      pack2<kBf16>(fmaf(s, acc[3][e], unpack_lo<kBf16>(b.w)), fmaf(s, acc[3][e + 1], unpack_hi<kBf16>(b.w))));
+}
+// rows without an adapter, columns n0 to n1 (multiples of 8)
+__device__ __forceinline__ void ad_copy(const AdapterArgs& a, const int4& tile, const int32_t* rows, int n0, int n1) {
+    const int pieces = max(0, n1 - n0) / 8;
+    for (int i = threadIdx.x; i < tile.z * pieces; i += kAdThreads) {
+        const int row = rows[i / pieces], col = n0 + i % pieces * 8;
+        *reinterpret_cast<uint4*>(const_cast<uint16_t*>(ad_row(a.out, row, a.ld_out)) + col) = *reinterpret_cast<const uint4*>(ad_row(a.base, row, a.ld_base) + col);
+    }
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------------
+// Each warp has a ring of its own for its groups of 32 rows of `up` (contiguous: one bulk copy each), filled from the start on: 4 groups up to rank
+// 16, 2 beyond. Longer rows than 64 values have no room, and go from memory to registers.
+constexpr int kAdRingRank = 64;
+__host__ __device__ constexpr int ad_ring_slots(int rank) { return rank > kAdRingRank ? 0 : rank <= 16 ? 4 : 2; }
+__host__ __device__ constexpr int ad_ring_bytes(int rank) { return ad_ring_slots(rank) * 32 * rank * 2; }
+// the sums of the eight CTAs, and before that of the warps; h; its two 16-bit parts
+template <int NT>
+__host__ __device__ constexpr size_t ad_few_smem_bytes(int rank) {
+    const int padded = (rank + NT * 8 - 1) / (NT * 8) * NT * 8;
+    return static_cast<size_t>(kAdWarps) * ad_ring_bytes(rank) + (static_cast<size_t>(2 * kAdWarps) * 16 * NT * 8 + 16 * padded) * 4 +
+           static_cast<size_t>(2) * 16 * ad_pitch(rank) * 2;
+}
+
+template <int NT, bool kBf16>
+__global__ void __launch_bounds__(kAdThreads, 2) adapter_few_kernel(const AdapterArgs a) {
+    constexpr int C = NT * 8;
+    extern __shared__ __align__(16) uint8_t ad_smem[];
+    __shared__ float row_scale[16];
+    __shared__ uint64_t full[kAdWarps][4];
+    const int rank = a.rank, padded = (rank + C - 1) / C * C, pitch = ad_pitch(rank), slots = ad_ring_slots(rank), ctas = a.cluster;
+    float* red = reinterpret_cast<float*>(ad_smem + kAdWarps * ad_ring_bytes(rank));      // [8 warps][16][C]
+    float* part = red + kAdWarps * 16 * C;                            // [8 CTAs][16][C]
+    float* h = part + kAdCluster * 16 * C;                            // [16][padded]
+    uint16_t* h_hi = reinterpret_cast<uint16_t*>(h + 16 * padded);    // [16][pitch]
+    uint16_t* h_lo = h_hi + 16 * pitch;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    // ---- ahead of the wait for what ran before: the plan, which no kernel writes ----
+    griddep_launch_dependents();
+    const uint32_t cta = ad_cta_rank();
+    const int index = blockIdx.x / ctas;
+    const int4 tile = a.tiles[index];
+    const int32_t* rows = a.tile_rows + index * kAdRows;
+    const int row0 = rows[g], row1 = rows[g + 8];
+    const int n_slice = (a.outputs + ctas * 32 - 1) / (ctas * 32) * 32, k_slice = (a.width + ctas * 32 - 1) / (ctas * 32) * 32;
+    const int n0 = static_cast<int>(cta) * n_slice, n1 = min(a.outputs, n0 + n_slice);
+    const int k0 = static_cast<int>(cta) * k_slice, k1 = min(a.width, k0 + k_slice);
+    if (tile.x < 0 || tile.x >= a.n_adapters) {        // (the whole cluster)
+        griddep_wait();
+        ad_copy(a, tile, rows, n0, n1);
+        return;
+    }
+    const uint16_t* up = reinterpret_cast<const uint16_t*>(a.up) + static_cast<int64_t>(tile.x) * a.outputs * rank;
+    const uint16_t* down = reinterpret_cast<const uint16_t*>(a.down) + static_cast<int64_t>(tile.x) * rank * a.width;
+    uint8_t* ring = ad_smem + warp * ad_ring_bytes(rank);
+    auto load = [&](int n, int slot) {       // (one lane) rows n to n + 31 of `up`, those that are mine
+        const uint32_t bytes = static_cast<uint32_t>(min(32, n1 - n)) * rank * 2;
+        mbar_expect_tx(&full[warp][slot], bytes);
+        bulk_load_1d(ring + slot * 64 * rank, up + static_cast<int64_t>(n) * rank, bytes, &full[warp][slot], kEvictFirst);
+    };
+    if (lane == 0) {
+        for (int i = 0; i < slots; ++i) mbar_init(&full[warp][i], 1);
+        fence_barrier_init();
+    }
+    __syncwarp();
+    griddep_wait();
+    ad_cluster_arrive();       // (the other CTAs' shared memory may be written from the wait on)
+    if (lane == 0)
+        for (int i = 0; i < slots; ++i)
+            if (n0 + (warp + i * kAdWarps) * 32 < n1) load(n0 + (warp + i * kAdWarps) * 32, i);
+    __syncwarp();
+    // my two rows of the tile (those that are not there repeat the last one)
+    const bool live0 = g < tile.z, live1 = g + 8 < tile.z;
+    const uint16_t *x0 = ad_row(a.x, row0, a.ld_x), *x1 = ad_row(a.x, row1, a.ld_x);
+    const float scale = a.scales[tile.x];
+    const uint16_t *b0 = ad_row(a.base, row0, a.ld_base) + t * 8, *b1 = ad_row(a.base, row1, a.ld_base) + t * 8;
+    uint4 next0 = ad_zero(), next1 = ad_zero();       // of base: one group ahead
+    auto ask = [&](int n) {
+        if (live0 && n + t * 8 < n1) next0 = *reinterpret_cast<const uint4*>(b0 + n);
+        if (live1 && n + t * 8 < n1) next1 = *reinterpret_cast<const uint4*>(b1 + n);
+    };
+    for (int rb = 0; rb < rank; rb += C) {
+        // ---- my part of the width, 32 columns at a time, shared out among the warps ----
+        float acc[NT][4];
+        ad_down<NT, kBf16, NT == 8 ? 1 : 2>(acc, x0, x1, down, rb, rank, a.width, k0, k1, warp, kAdWarps, g, t);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            *reinterpret_cast<float2*>(red + (warp * 16 + g) * C + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+            *reinterpret_cast<float2*>(red + (warp * 16 + g + 8) * C + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
+        }
+        if (rb == 0) ask(n0 + warp * 32);
+        __syncthreads();
+        if (rb == 0) ad_cluster_wait();      // all have begun
+        // ---- to everybody, and added up there in the order of the CTAs ----
+        for (int i = tid; i < 16 * C / 4; i += kAdThreads) {
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kAdWarps; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(red + w * 16 * C + i * 4);
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            for (int p = 0; p < ctas; ++p) ad_store4(ad_at(part + cta * 16 * C + i * 4, p), s);
+        }
+        ad_cluster_arrive();
+        ad_cluster_wait();
+        for (int i = tid; i < 16 * C; i += kAdThreads) {
+            float s = 0.0f;
+            for (int p = 0; p < ctas; ++p) s += part[p * 16 * C + i];
+            h[i / C * padded + rb + i % C] = s;
+        }
+        if (rb + C < rank) {                 // nobody sends the next ones before these are taken
+            ad_cluster_arrive();
+            ad_cluster_wait();
+        }
+    }
+    __syncthreads();
     if constexpr (!kBf16) {
-        for (int r = warp; r < M; r += kAdWarps) {
+        for (int r = warp; r < 16; r += kAdWarps) {
             float m = 0.0f;
             for (int c = lane; c < rank; c += 32) m = fmaxf(m, fabsf(h[r * padded + c]));
             m = warp_max(m);
-            int e = 0;
-            if (m > 0.0f && m < INFINITY) frexpf(m, &e);
-            if (lane == 0) row_scale[r] = ldexpf(1.0f, min(max(e - 9, -126), 126));
+            const float2 f = ad_row_scale(m);
+            for (int c = lane; c < rank; c += 32) h[r * padded + c] *= f.x;
+            if (lane == 0) row_scale[r] = f.y;
         }
         __syncthreads();
     }
     const int k_steps = (rank + 15) / 16;
-    for (int i = tid; i < M * k_steps * 16; i += kAdThreads) {
+    for (int i = tid; i < 16 * k_steps * 16; i += kAdThreads) {
         const int r = i / (k_steps * 16), c = i % (k_steps * 16);
-        float v = c < rank ? h[r * padded + c] : 0.0f;
-        if constexpr (!kBf16) v /= row_scale[r];
-        const uint32_t hi = pack2<kBf16>(v, 0.0f);
-        const float rest = v - unpack_lo<kBf16>(hi);
-        h_hi[r * pitch + c] = static_cast<uint16_t>(hi);
-        h_lo[r * pitch + c] = static_cast<uint16_t>(pack2<kBf16>(fabsf(rest) < INFINITY ? rest : 0.0f, 0.0f));
+        ad_split<kBf16>(c < rank ? h[r * padded + c] : 0.0f, h_hi[r * pitch + c], h_lo[r * pitch + c]);
     }
     __syncthreads();
-    // ---- 3. my eighth of the outputs, 32 columns at a time. Tile j, column 2 t + e of the MMA is column 8 t + 2 j + e of the 32 ----
-    const uint16_t* up = reinterpret_cast<const uint16_t*>(a.up) + static_cast<int64_t>(tile.x) * a.outputs * rank;
-    const float scale = a.scales[tile.x];
-    float s0 = scale, s1 = scale;
-    if constexpr (!kBf16) {
-        s0 *= row_scale[r0];
-        s1 *= row_scale[r1];
-    }
-    for (int n = n0 + kw * 32; n < n1; n += KW * 32) {
-        const int col = n + t * 8;
-        const bool in = col < n1;
-        const uint16_t* b0 = reinterpret_cast<const uint16_t*>(a.base) + row0 * a.ld_base + col;
-        const uint16_t* b1 = reinterpret_cast<const uint16_t*>(a.base) + row1 * a.ld_base + col;
-        const uint4 base0 = in && live0 ? *reinterpret_cast<const uint4*>(b0) : ad_zero();
-        const uint4 base1 = in && live1 ? *reinterpret_cast<const uint4*>(b1) : ad_zero();
-        float acc[4][4];
+    // ---- my part of the outputs, 32 columns at a time ----
+    const float s0 = kBf16 ? scale : scale * row_scale[g], s1 = kBf16 ? scale : scale * row_scale[g + 8];
+    uint16_t *o0 = const_cast<uint16_t*>(ad_row(a.out, row0, a.ld_out)) + t * 8, *o1 = const_cast<uint16_t*>(ad_row(a.out, row1, a.ld_out)) + t * 8;
+    const int first = (g >> 1) * 8 + (g & 1);                 // my row of `up` in a group of 32
+    const uint16_t* my_up = up + static_cast<int64_t>(first) * rank + t * 4;
+    int slot = 0;
+    uint32_t phase = 0;
+    for (int n = n0 + warp * 32; n < n1; n += kAdWarps * 32) {
+        const bool in = n + t * 8 < n1;
+        const uint4 base0 = next0, base1 = next1;
+        ask(n + kAdWarps * 32);
+        float acc[4][4] = {};
+        if (slots > 0) {
+            mbar_wait(&full[warp][slot], phase);
+            const uint16_t* p = reinterpret_cast<const uint16_t*>(ring + slot * 64 * rank) + first * rank + t * 4;     // (rows that are not there: whatever the slot holds)
+            for (int c = 0; c < rank; c += 16) {
+                uint2 u[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-        const int up_row = n + (g >> 1) * 8 + (g & 1);
-        for (int ks = 0; ks < k_steps; ++ks) {
-            const int c = ks * 16 + t * 4;
-            uint2 u[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                u[j] = up_row + 2 * j < n1 && c < rank ? *reinterpret_cast<const uint2*>(up + static_cast<int64_t>(up_row + 2 * j) * rank + c)
-                                                       : make_uint2(0u, 0u);
-            const uint2 p0 = *reinterpret_cast<const uint2*>(h_hi + r0 * pitch + c), p1 = *reinterpret_cast<const uint2*>(h_hi + r1 * pitch + c);
-            const uint2 l0 = *reinterpret_cast<const uint2*>(h_lo + r0 * pitch + c), l1 = *reinterpret_cast<const uint2*>(h_lo + r1 * pitch + c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                mma_m16n8k16<kBf16>(acc[j], p0.x, p1.x, p0.y, p1.y, u[j].x, u[j].y);
-                mma_m16n8k16<kBf16>(acc[j], l0.x, l1.x, l0.y, l1.y, u[j].x, u[j].y);
+                for (int j = 0; j < 4; ++j) u[j] = c + t * 4 < rank ? *reinterpret_cast<const uint2*>(p + 2 * j * rank + c) : make_uint2(0u, 0u);
+                ad_up_step<kBf16>(acc, h_hi, h_lo, pitch, g, c + t * 4, u);
+            }
+            __syncwarp();       // (the slot has been read)
+            if (lane == 0 && n + slots * kAdWarps * 32 < n1) load(n + slots * kAdWarps * 32, slot);
+            if (++slot == slots) {
+                slot = 0;
+                phase ^= 1;
+            }
+        } else {
+            const uint16_t* p = my_up + static_cast<int64_t>(n) * rank;
+            for (int c = 0; c < rank; c += 16) {
+                uint2 u[4];
+                ad_up_load(u, p + c, rank, n1 - n - first, c + t * 4 < rank);
+                ad_up_step<kBf16>(acc, h_hi, h_lo, pitch, g, c + t * 4, u);
             }
         }
-        auto join = [&](const uint4& b, int e, float s) {
-            return make_uint4(pack2<kBf16>(fmaf(s, acc[0][e], unpack_lo<kBf16>(b.x)), fmaf(s, acc[0][e + 1], unpack_hi<kBf16>(b.x))),
-                              pack2<kBf16>(fmaf(s, acc[1][e], unpack_lo<kBf16>(b.y)), fmaf(s, acc[1][e + 1], unpack_hi<kBf16>(b.y))),
-                              pack2<kBf16>(fmaf(s, acc[2][e], unpack_lo<kBf16>(b.z)), fmaf(s, acc[2][e + 1], unpack_hi<kBf16>(b.z))),
-                              pack2<kBf16>(fmaf(s, acc[3][e], unpack_lo<kBf16>(b.w)), fmaf(s, acc[3][e + 1], unpack_hi<kBf16>(b.w))));
-        };
-        if (in && live0) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row0 * a.ld_out + col) = join(base0, 0, s0);
-        if (in && live1) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row1 * a.ld_out + col) = join(base1, 2, s1);
+        if (in && live0) *reinterpret_cast<uint4*>(o0 + n) = ad_join<kBf16>(base0, acc, 0, s0);
+        if (in && live1) *reinterpret_cast<uint4*>(o1 + n) = ad_join<kBf16>(base1, acc, 2, s1);
     }
 }
 
-template <int MT, int NT, bool kBf16>
-static int launch_adapters_as(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
-    auto kern = adapter_kernel<MT, NT, kBf16>;
+// ---- many rows -------------------------------------------------------------------------------------------------------------
+// tiles of 16 rows that a tile of so many rows has: 1, 2 or 4, so that they divide the warps
+__device__ __forceinline__ int ad_m_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+template <int NT, bool kBf16>
+__global__ void __launch_bounds__(kAdThreads, 2) adapter_down_kernel(const AdapterArgs a) {
+    constexpr int C = NT * 8;
+    __shared__ __align__(16) float red[kAdWarps][16][C];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int4 tile = a.tiles[blockIdx.x];
+    const int32_t* rows = a.tile_rows + blockIdx.x * kAdRows;
+    const int m_tiles = ad_m_tiles(tile.z), mt = warp % m_tiles, kw = warp / m_tiles, k_warps = kAdWarps / m_tiles;
+    const uint16_t *x0 = ad_row(a.x, rows[mt * 16 + g], a.ld_x), *x1 = ad_row(a.x, rows[mt * 16 + g + 8], a.ld_x);
+    // (in this order: the second kernel, which may start from here on, reads what came before this one without a wait)
+    griddep_wait();
+    griddep_launch_dependents();
+    if (tile.x < 0 || tile.x >= a.n_adapters) return;
+    const int k0 = blockIdx.y * a.k_part, k1 = min(a.width, k0 + a.k_part);
+    const uint16_t* down = reinterpret_cast<const uint16_t*>(a.down) + static_cast<int64_t>(tile.x) * a.rank * a.width;
+    float* h = a.h + (static_cast<int64_t>(blockIdx.y) * a.rows + tile.y) * a.rank;
+    for (int rb = 0; rb < a.rank; rb += C) {
+        float acc[NT][4];
+        ad_down<NT, kBf16, NT == 8 ? 2 : NT == 4 ? 3 : 4>(acc, x0, x1, down, rb, a.rank, a.width, k0, k1, kw, k_warps, g, t);
+        if (rb > 0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            *reinterpret_cast<float2*>(&red[warp][g][j * 8 + 2 * t]) = make_float2(acc[j][0], acc[j][1]);
+            *reinterpret_cast<float2*>(&red[warp][g + 8][j * 8 + 2 * t]) = make_float2(acc[j][2], acc[j][3]);
+        }
+        __syncthreads();
+        for (int i = tid; i < tile.z * C / 4; i += kAdThreads) {
+            const int r = i / (C / 4), c = i % (C / 4) * 4;
+            if (rb + c >= a.rank) continue;
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int w = 0; w < k_warps; ++w) {
+                const float4 v = *reinterpret_cast<const float4*>(&red[w * m_tiles + (r >> 4)][r & 15][c]);
+                s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+            }
+            *reinterpret_cast<float4*>(h + static_cast<int64_t>(r) * a.rank + rb + c) = s;
+        }
+    }
+}
+
+// KS: k-steps of 16 whose part of `up` a warp has in registers at once. CTA y of a tile has the groups of 256 outputs y, y + gridDim.y, ...
+template <int KS, bool kBf16>
+__global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const AdapterArgs a) {
+    extern __shared__ __align__(16) uint8_t ad_smem[];
+    __shared__ float row_scale[kAdRows];
+    __shared__ int rows[kAdRows];
+    const int rank = a.rank, pitch = ad_pitch(rank), k_steps = (rank + 15) / 16;
+    uint16_t* h_hi = reinterpret_cast<uint16_t*>(ad_smem);            // [64][pitch]
+    uint16_t* h_lo = h_hi + kAdRows * pitch;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int4 tile = a.tiles[blockIdx.x];
+    const int n_step = gridDim.y * kAdCols;
+    int n = blockIdx.y * kAdCols + warp * 32;
+    if (tile.x < 0 || tile.x >= a.n_adapters) {
+        pdl_enter();
+        for (int c = blockIdx.y * kAdCols; c < a.outputs; c += n_step) ad_copy(a, tile, a.tile_rows + blockIdx.x * kAdRows, c, min(a.outputs, c + kAdCols));
+        return;
+    }
+    // ---- what does not need h: all of it was there before the first kernel let this one start ----
+    const int m_tiles = ad_m_tiles(tile.z);
+    const uint16_t* up = reinterpret_cast<const uint16_t*>(a.up) + static_cast<int64_t>(tile.x) * a.outputs * rank;
+    if (tid < kAdRows) rows[tid] = a.tile_rows[blockIdx.x * kAdRows + tid];
+    const float scale = a.scales[tile.x];
+    uint2 u[KS][4];
+    uint4 base[kAdRows / 16][2];
+    const int first = (g >> 1) * 8 + (g & 1);                 // my row of `up` in a group of 32
+    const uint16_t* my_up = up + static_cast<int64_t>(first) * rank + t * 4;
+    auto ask = [&](int at) {        // the first k-steps of `up` and all of base, for the 32 outputs from `at` on
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) ad_up_load(u[ks], my_up + static_cast<int64_t>(at) * rank + ks * 16, rank, a.outputs - at - first, ks * 16 + t * 4 < rank);
+        if (at + t * 8 < a.outputs) {
+#pragma unroll
+            for (int m = 0; m < kAdRows / 16; ++m)
+                if (m < m_tiles) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) base[m][e] = *reinterpret_cast<const uint4*>(ad_row(a.base, rows[m * 16 + g + 8 * e], a.ld_base) + at + t * 8);
+                }
+        }
+    };
+    __syncthreads();
+    ask(n);
+    griddep_wait();
+    griddep_launch_dependents();
+    // ---- h, summed over the parts of the width: four values per thread, a row's in neighbouring ones (of a power of two of lanes) ----
+    const float* h = a.h + static_cast<int64_t>(tile.y) * rank;
+    const int64_t part = static_cast<int64_t>(a.rows) * rank;
+    const int quads = k_steps * 4;                                     // of a row, the last two behind an odd rank / 8
+    if constexpr (kBf16) {
+        for (int i = tid; i < m_tiles * 16 * quads; i += kAdThreads) {
+            const int r = i / quads, c = i % quads * 4;
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < tile.z && c < rank)
+                for (int p = 0; p < a.k_parts; ++p) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(h + p * part + static_cast<int64_t>(r) * rank + c));
+                    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+                }
+            const uint32_t h0 = pack2<true>(s.x, s.y), h1 = pack2<true>(s.z, s.w);
+            auto rest = [](float v, float hi) { const float d = v - hi; return fabsf(d) < INFINITY ? d : 0.0f; };
+            *reinterpret_cast<uint2*>(h_hi + r * pitch + c) = make_uint2(h0, h1);
+            *reinterpret_cast<uint2*>(h_lo + r * pitch + c) = make_uint2(pack2<true>(rest(s.x, bf16_lo(h0)), rest(s.y, bf16_hi(h0))),
+                                                                         pack2<true>(rest(s.z, bf16_lo(h1)), rest(s.w, bf16_hi(h1))));
+        }
+    } else {          // a warp has whole rows, for their largest values
+        for (int r = warp; r < m_tiles * 16; r += kAdWarps) {
+            float v[kAdMaxRank / 32], m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kAdMaxRank / 32; ++i) {
+                const int c = i * 32 + lane;
+                v[i] = 0.0f;
+                if (i * 32 >= rank) break;
+                if (r < tile.z && c < rank)
+                    for (int p = 0; p < a.k_parts; ++p) v[i] += __ldcg(h + p * part + static_cast<int64_t>(r) * rank + c);
+                m = fmaxf(m, fabsf(v[i]));
+            }
+            const float2 f = ad_row_scale(warp_max(m));
+            if (lane == 0) row_scale[r] = f.y;
+#pragma unroll
+            for (int i = 0; i < kAdMaxRank / 32; ++i) {
+                const int c = i * 32 + lane;
+                if (i * 32 >= k_steps * 16) break;
+                if (c < k_steps * 16) ad_split<kBf16>(v[i] * f.x, h_hi[r * pitch + c], h_lo[r * pitch + c]);
+            }
+        }
+    }
+    __syncthreads();
+    for (; n - warp * 32 < a.outputs; n += n_step) {       // (a warp whose 32 are behind the end asks for nothing and writes nothing)
+        const int col = n + t * 8;
+#pragma unroll
+        for (int m = 0; m < kAdRows / 16; ++m) {
+            if (m >= m_tiles) break;
+            const int r0 = m * 16 + g;
+            float acc[4][4] = {};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                if (ks < k_steps) ad_up_step<kBf16>(acc, h_hi, h_lo, pitch, r0, ks * 16 + t * 4, u[ks]);
+            for (int ks = KS; ks < k_steps; ++ks) {
+                uint2 more[4];
+                ad_up_load(more, my_up + static_cast<int64_t>(n) * rank + ks * 16, rank, a.outputs - n - first, ks * 16 + t * 4 < rank);
+                ad_up_step<kBf16>(acc, h_hi, h_lo, pitch, r0, ks * 16 + t * 4, more);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (col < a.outputs && r0 + 8 * e < tile.z)
+                    *reinterpret_cast<uint4*>(const_cast<uint16_t*>(ad_row(a.out, rows[r0 + 8 * e], a.ld_out)) + col) =
+                        ad_join<kBf16>(base[m][e], acc, 2 * e, kBf16 ? scale : scale * row_scale[r0 + 8 * e]);
+        }
+        ask(n + n_step);
+    }
+}
+
+template <int NT, bool kBf16>
+static int launch_few(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
+    auto kern = adapter_few_kernel<NT, kBf16>;
     static bool configured[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        HDS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ad_smem_bytes<MT>(kAdMaxRank))));
+        HDS_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(ad_few_smem_bytes<NT>(NT == 2 ? 16 : NT == 4 ? 32 : kAdRingRank) > ad_few_smem_bytes<NT>(kAdMaxRank)
+                                                                  ? ad_few_smem_bytes<NT>(NT == 2 ? 16 : NT == 4 ? 32 : kAdRingRank)
+                                                                  : ad_few_smem_bytes<NT>(kAdMaxRank))));
         configured[dev & 63] = true;
     }
-    HDS_CHECK_CUDA(launch_kernel_cluster(kern, kAdCluster, dim3(static_cast<unsigned>(n_tiles) * kAdCluster), dim3(kAdThreads),
-                                         ad_smem_bytes<MT>(a.rank), s, a));
+    HDS_CHECK_CUDA(launch_kernel_cluster(kern, a.cluster, dim3(static_cast<unsigned>(n_tiles) * a.cluster), dim3(kAdThreads),
+                                         ad_few_smem_bytes<NT>(a.rank), s, a));
     return HDS_OK;
 }
 
-template <int MT, bool kBf16>
-static int launch_adapters(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
-    return a.rank <= 16 ? launch_adapters_as<MT, 2, kBf16>(a, n_tiles, s)
-           : a.rank <= 32 ? launch_adapters_as<MT, 4, kBf16>(a, n_tiles, s) : launch_adapters_as<MT, 8, kBf16>(a, n_tiles, s);
+template <int NT, int KS, bool kBf16>
+static int launch_many(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
+    auto up = adapter_up_kernel<KS, kBf16>;
+    const size_t smem = static_cast<size_t>(2) * kAdRows * ad_pitch(a.rank) * 2;
+    static bool configured[64] = {false};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured[dev & 63]) {
+        HDS_CHECK_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kAdRows * ad_pitch(kAdMaxRank) * 2));
+        configured[dev & 63] = true;
+    }
+    HDS_CHECK_CUDA(launch_kernel(adapter_down_kernel<NT, kBf16>, dim3(n_tiles, a.k_parts), dim3(kAdThreads), 0, s, a));
+    // CTAs of a tile: the fewest waves of two per SM, a CTA's beginning and end counted as one group of outputs
+    const int groups = (a.outputs + kAdCols - 1) / kAdCols, slots = 2 * sm_count();
+    int parts = 1;
+    int64_t best = INT64_MAX;
+    for (int p = 1; p <= groups; ++p) {
+        const int64_t cost = (static_cast<int64_t>(n_tiles) * p + slots - 1) / slots * ((groups + p - 1) / p + 1);
+        if (cost < best) {
+            best = cost;
+            parts = p;
+        }
+        if (static_cast<int64_t>(n_tiles) * p >= slots && p >= 8) break;
+    }
+    HDS_CHECK_CUDA(launch_kernel(up, dim3(n_tiles, parts), dim3(kAdThreads), smem, s, a));
+    return HDS_OK;
+}
+
+template <bool kBf16>
+static int launch_adapters(const AdapterArgs& a, int n_tiles, bool few, cudaStream_t s) {
+    if (few)
+        return a.rank <= 16 ? launch_few<2, kBf16>(a, n_tiles, s) : a.rank <= 32 ? launch_few<4, kBf16>(a, n_tiles, s) : launch_few<8, kBf16>(a, n_tiles, s);
+    return a.rank <= 16 ? launch_many<2, 1, kBf16>(a, n_tiles, s) : a.rank <= 32 ? launch_many<4, 2, kBf16>(a, n_tiles, s) : launch_many<8, 4, kBf16>(a, n_tiles, s);
 }
 
 }  // namespace hds
 
 using namespace hds;
 
+// Parts of the width of the first of two kernels: two CTAs on every SM, of at least 256 columns each.
+extern "C" int hds_adapter_parts(int n_tiles, int width) {
+    const int most = (width + 255) / 256;
+    int parts = n_tiles > 0 ? (2 * sm_count() + n_tiles / 2) / n_tiles : 1;
+    parts = parts < 1 ? 1 : parts > most ? most : parts;
+    return parts > 32 ? 32 : parts;
+}
+
 extern "C" int hds_adapter_add(const void* base, int64_t ld_base, const void* x, int64_t ld_x, const void* down, const void* up, const float* scales,
-                               int n_adapters, int rank, int width, int outputs, const int32_t* order, const int32_t* tiles, int n_tiles,
-                               int tile_rows, void* out, int64_t ld_out, int dtype, void* stream) {
+                               int n_adapters, int rank, int width, int outputs, int rows, const int32_t* tiles, const int32_t* tile_rows, int n_tiles,
+                               int most_rows, void* out, int64_t ld_out, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
     HDS_REQUIRE(dtype == 0 || dtype == 1, "adapter_add: dtype must be 0 (bf16) or 1 (fp16)");
     HDS_REQUIRE(rank >= 8 && rank <= kAdMaxRank && rank % 8 == 0, "adapter_add: ranks are multiples of 8 up to 256");
-    HDS_REQUIRE(width > 0 && outputs > 0 && width % 8 == 0 && outputs % 8 == 0, "adapter_add: widths are multiples of 8");
+    HDS_REQUIRE(width > 0 && outputs > 0 && width % 8 == 0 && outputs % 8 == 0 && width < (1 << 24) && outputs < (1 << 24),
+                "adapter_add: widths are multiples of 8 below 2^24");
     HDS_REQUIRE(ld_base % 8 == 0 && ld_x % 8 == 0 && ld_out % 8 == 0, "adapter_add: rows start on 16-byte boundaries");
+    HDS_REQUIRE(ld_base >= 0 && ld_x >= 0 && ld_out >= 0 && ld_base < (1 << 30) && ld_x < (1 << 30) && ld_out < (1 << 30), "adapter_add: rows are less than 2^30 apart");
     HDS_REQUIRE(((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(down) |
                   reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(tiles)) & 15) == 0,
                 "adapter_add: operands start on 16-byte boundaries");
-    HDS_REQUIRE(tile_rows == 16 || tile_rows == 64, "adapter_add: tiles of 16 or 64 rows");
-    HDS_REQUIRE(n_tiles >= 0 && n_tiles <= (1 << 26), "adapter_add: too many tiles");
+    HDS_REQUIRE(most_rows >= 0 && most_rows <= kAdRows, "adapter_add: tiles of up to 64 rows");
+    HDS_REQUIRE(n_tiles >= 0 && n_tiles <= (1 << 26) && rows >= 0, "adapter_add: too many tiles");
     if (n_tiles == 0) return HDS_OK;
     AdapterArgs a;
     memset(&a, 0, sizeof(a));
-    a.x = x; a.base = base; a.out = out; a.ld_x = ld_x; a.ld_base = ld_base; a.ld_out = ld_out;
-    a.down = down; a.up = up; a.scales = scales; a.order = order; a.tiles = reinterpret_cast<const int4*>(tiles);
-    a.n_adapters = n_adapters; a.rank = rank; a.width = width; a.outputs = outputs;
+    a.x = x; a.base = base; a.out = out;
+    a.ld_x = static_cast<int>(ld_x); a.ld_base = static_cast<int>(ld_base); a.ld_out = static_cast<int>(ld_out);
+    a.down = down; a.up = up; a.scales = scales; a.tiles = reinterpret_cast<const int4*>(tiles); a.tile_rows = tile_rows;
+    a.n_adapters = n_adapters; a.rank = rank; a.width = width; a.outputs = outputs; a.rows = rows;
+    const bool few = workspace == nullptr;
+    HDS_REQUIRE(!few || most_rows <= kAdFew, "adapter_add: tiles of more than 16 rows need a workspace");
+    a.cluster = getenv("HDS_ADC") ? atoi(getenv("HDS_ADC")) : n_tiles * 8 <= sm_count() ? 8 : 4;
+    if (!few) {
+        const int parts = hds_adapter_parts(n_tiles, width);
+        a.k_part = ((width + parts - 1) / parts + 31) / 32 * 32;
+        a.k_parts = (width + a.k_part - 1) / a.k_part;
+        HDS_REQUIRE(workspace_bytes >= static_cast<int64_t>(parts) * rows * rank * 4 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+                    "adapter_add: workspace too small");
+        a.h = static_cast<float*>(workspace);
+    }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tile_rows == 16) return dtype == 0 ? launch_adapters<1, true>(a, n_tiles, s) : launch_adapters<1, false>(a, n_tiles, s);
-    return dtype == 0 ? launch_adapters<4, true>(a, n_tiles, s) : launch_adapters<4, false>(a, n_tiles, s);
+    return dtype == 0 ? launch_adapters<true>(a, n_tiles, few, s) : launch_adapters<false>(a, n_tiles, few, s);
 }

@@ -17,7 +17,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import native
-from .plans import AdapterPlan, SharedPrefixPlan  # noqa: F401
+from .plans import ADAPTER_FEW, AdapterPlan, SharedPrefixPlan  # noqa: F401
 
 ACT_IDENTITY, ACT_GELU, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_SWIGLU_CLAMPED, ACT_RELU2 = 0, 1, 2, 3, 4, 5, 6
 ACT_CODES = {"identity": 0, None: 0, "gelu": 1, "relu": 2, "silu": 3, "gelu_tanh": 4, "gelu_new": 4,
@@ -973,6 +973,8 @@ def retention_stuck() -> bool:
 # (A step makes hundreds of these calls: their checks read each attribute once, and a stream is asked for by its number. A Stream object and
 # a device guard alone cost 5 us of the 22 that a call took; it takes 9 to 12 so.)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+import os
+_ADAPTER_TWO = int(os.environ.get('HDS_ADTWO', '0'))
 
 
 def _place(t: torch.Tensor, name: str) -> int:
@@ -1042,15 +1044,20 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
     if plan.index != index:
         raise ValueError(f"the plan is on {plan.device}, the call is on cuda:{index}")
     p_base, p_out = base.data_ptr(), out.data_ptr()
-    fn = native.cuda_lib().hds_adapter_add
+    count = plan.n_tiles if p_out == p_base and ld_out == ld_base else plan.n_tiles_and_bare
+    if count == 0:
+        return out
+    lib = native.cuda_lib()
     with _On(index):
-        stream = _raw_stream(index)
-        for height, tiles, count in plan.launches if p_out != p_base or ld_out != ld_base else plan.launches_in_place:
-            rc = fn(p_base, ld_base, x.data_ptr(), ld_x, down.data_ptr(), up.data_ptr(), scales.data_ptr(), n, R, K, N, plan.order_ptr, tiles, count, height,
-                    p_out, ld_out, dt, stream)
-            if rc:
-                native.check(rc, "hds_adapter_add")
-            _count()
+        ws, n_bytes = None, 0
+        if plan.tile_rows > ADAPTER_FEW or _ADAPTER_TWO:
+            n_bytes = lib.hds_adapter_parts(count, K) * T * R * 4
+            ws = x.new_empty(n_bytes // 2)       # of this call alone: a plan may be in use on several streams, and in graphs
+        rc = lib.hds_adapter_add(p_base, ld_base, x.data_ptr(), ld_x, down.data_ptr(), up.data_ptr(), scales.data_ptr(), n, R, K, N, T,
+                                 plan.tiles_ptr, plan.rows_ptr, count, plan.tile_rows, p_out, ld_out, _p(ws), n_bytes, dt, _raw_stream(index))
+    if rc:
+        native.check(rc, "hds_adapter_add")
+    _count(1 if ws is None else 2)
     return out
 
 

@@ -62,7 +62,8 @@ def _declare_cuda(lib: ctypes.CDLL, partial: bool = False) -> None:
         "hds_retention": [P, P, L, P, P, L, P, P, P, F, I, P, P, I, I, I, I, I, I, P, L, P, L, F, P, L, I, P, I, P],
         "hds_linear_attention": [P, P, P, P, L, P, L, P, F, P, P, I, I, I, I, I, I, P, L, P, L, P, F, P, L, I, P, I, P],
         "hds_gemm_next_act_limit": [F],
-        "hds_adapter_add": [P, L, P, L, P, P, P, I, I, I, I, P, P, I, I, P, L, I, P],
+        "hds_adapter_add": [P, L, P, L, P, P, P, I, I, I, I, I, P, P, I, I, P, L, P, L, I, P],
+        "hds_adapter_parts": [I, I],
         "hds_paged_attention_shared": [P, L, P, L, I, P, L, P, I, P, I, I, P, I, I, I, I, I, I, I, F, P, L, I, P],
         "hds_logit_controls": [P, L, P, L, I, I, P, L, I, P, P, P, P, P, P, L, P, L, I, P, L, I, P, I, P],
         "hds_moe_table_route": [P, P, I, I, I, I, P, P, P, P, P],

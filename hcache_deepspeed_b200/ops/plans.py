@@ -9,10 +9,8 @@ from typing import Sequence, Tuple
 import numpy as np
 import torch
 
-#: rows of a small and of a large tile of the adapter kernel
-ADAPTER_SMALL, ADAPTER_LARGE = 16, 64
-#: rows of one adapter that still go as small tiles
-ADAPTER_FEW = 32
+#: rows of a tile of the adapter kernels, and of the tiles that go through one kernel
+ADAPTER_ROWS, ADAPTER_FEW = 64, 16
 
 
 def _host_ints(values, name: str) -> np.ndarray:
@@ -38,36 +36,23 @@ class AdapterPlan:
         #: rows sorted by adapter, those without one first
         order = np.argsort(self.ids, kind="stable").astype(np.int32)
         names, starts, counts = np.unique(self.ids[order], return_index=True, return_counts=True)
-        tiles = {ADAPTER_SMALL: [], ADAPTER_LARGE: []}
-        for name, start, count in zip(names.tolist(), starts.tolist(), counts.tolist()):
-            if name < 0:
-                continue
-            stop = start + count
-            while start < stop:
-                left = stop - start
-                rows = ADAPTER_SMALL if left <= ADAPTER_FEW else ADAPTER_LARGE
-                tiles[rows].append((name, start, min(rows, left), 0))
-                start += rows
-        n_bare = int((self.ids < 0).sum())
-        #: tiles of rows without an adapter (they are copied, whatever the tile's size), behind the others of one of the two lists
-        bare = [(-1, i, min(ADAPTER_LARGE, n_bare - i), 0) for i in range(0, n_bare, ADAPTER_LARGE)]
-        host = ADAPTER_LARGE if tiles[ADAPTER_LARGE] else ADAPTER_SMALL
-        self._parts = [(rows, tiles[rows] + (bare if rows == host else []), len(bare) if rows == host else 0) for rows in (ADAPTER_LARGE, ADAPTER_SMALL)]
+        bounds = [(name, start, start + count) for name, start, count in zip(names.tolist(), starts.tolist(), counts.tolist())]
+        cut = lambda name, start, stop: [(name, p, min(ADAPTER_ROWS, stop - p), 0) for p in range(start, stop, ADAPTER_ROWS)]  # noqa: E731
+        #: (adapter, first place in the order, rows, 0); rows without an adapter (they are copied) come last
+        tiles = [t for b in bounds if b[0] >= 0 for t in cut(*b)]
+        self.n_tiles = len(tiles)
+        self.tile_rows = max((t[2] for t in tiles), default=0)
+        tiles += [t for b in bounds if b[0] < 0 for t in cut(*b)]
+        self.n_tiles_and_bare = len(tiles)
+        self.tiles = tiles
         self.device = None if device is None else torch.device(device)
-        #: device number (-1: not on a GPU); launches: (tile rows, device pointer of the tiles, their number), with and without the rows that are copied
-        self.index, self.launches, self.launches_in_place = -1, [], []
+        #: device number (-1: not on a GPU) and device pointers
+        self.index, self.tiles_ptr, self.rows_ptr = -1, 0, 0
         if self.device is not None and self.device.type == "cuda":
-            pad = -order.size % 4        # tiles start on 16-byte boundaries
-            flat = [order, np.zeros(pad, dtype=np.int32)] + [np.asarray(t, dtype=np.int32).reshape(-1) for _, t, _ in self._parts]
-            self._dev = torch.from_numpy(np.concatenate(flat)).to(self.device)
-            self.index, self.order_ptr = self._dev.get_device(), self._dev.data_ptr()
-            at = self.order_ptr + 4 * (order.size + pad)
-            for rows, t, n_bare in self._parts:
-                if t:
-                    self.launches.append((rows, at, len(t)))
-                if len(t) > n_bare:
-                    self.launches_in_place.append((rows, at, len(t) - n_bare))
-                at += 16 * len(t)
+            places = np.asarray([[min(start + r, start + n - 1) for r in range(ADAPTER_ROWS)] for _, start, n, _ in tiles], dtype=np.int64).reshape(-1, ADAPTER_ROWS)
+            self._dev = torch.from_numpy(np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), order[places].reshape(-1)])).to(self.device)
+            self.index, self.tiles_ptr = self._dev.get_device(), self._dev.data_ptr()
+            self.rows_ptr = self.tiles_ptr + 16 * len(tiles)
 
 
 class SharedPrefixPlan:

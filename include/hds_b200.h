@@ -534,11 +534,14 @@ int hds_retention_status(int* stuck);
 
 /* Low-rank adapters of many requests beside a shared projection: out[t] = base[t] + scales[i] * (x[t] down[i]^T) up[i]^T. down
  * [n_adapters][rank][width], up [n_adapters][outputs][rank], 16-bit (dtype 0 bf16, 1 fp16); scales fp32; rank, width and outputs multiples of 8,
- * rank <= 256. order: rows sorted by adapter; tiles int32 [n_tiles][4] = (adapter, first place in order, rows <= tile_rows, 0), an adapter of
- * -1 copying base (any number of rows). tile_rows 16 or 64. out may be base. All rows on 16-byte boundaries. */
+ * rank <= 256. tiles int32 [n_tiles][4] = (adapter, place of the first row among the rows sorted by adapter, rows, 0), an adapter of -1 copying
+ * base; tile_rows int32 [n_tiles][64]: a tile's rows, the last one repeated to the end (neither is written by a kernel that may still run).
+ * most_rows: rows of the largest tile with an adapter, up to 64; beyond 16 it needs a workspace of hds_adapter_parts(n_tiles, width) * rows *
+ * rank * 4 bytes (nothing in it outlives the call), with which two kernels run instead of one. out may be base. All rows on 16-byte boundaries. */
 int hds_adapter_add(const void* base, int64_t ld_base, const void* x, int64_t ld_x, const void* down, const void* up, const float* scales,
-                    int n_adapters, int rank, int width, int outputs, const int32_t* order, const int32_t* tiles, int n_tiles, int tile_rows,
-                    void* out, int64_t ld_out, int dtype, void* stream);
+                    int n_adapters, int rank, int width, int outputs, int rows, const int32_t* tiles, const int32_t* tile_rows, int n_tiles,
+                    int most_rows, void* out, int64_t ld_out, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+int hds_adapter_parts(int n_tiles, int width);
 
 /* Paged attention of a batch whose sequences share prefixes. q and out: rows of n_q_heads * head_dim values, ld_q / ld_out apart; a group of
  * neighbouring sequences reads its prefix once. tiles int32 [n_tiles][4] = (sequence whose table names the prefix' pages, first row, tokens <=

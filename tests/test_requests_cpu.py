@@ -13,17 +13,13 @@ from hcache_deepspeed_b200.ops.backend import CpuOps
 
 
 # ---- adapters --------------------------------------------------------------------------------------------------------
-def _tiles(plan):
-    return [(rows, t) for rows, tiles, _ in plan._parts for t in tiles]
-
-
 @pytest.mark.parametrize("ids", [[], [0], [-1], [-1, -1, 3], [2, 0, 2, 0, 2], list(range(5)) * 30, [1] * 33, [1] * 97 + [-1] * 130 + [0] * 3, [4] * 200])
 def test_every_row_is_in_one_tile_of_its_adapter(ids):
     plan = kernels.AdapterPlan(ids, 5)
     order = sorted(range(len(ids)), key=lambda i: (max(ids[i], -1), i))
     seen = []
-    for rows, (name, start, n, _) in _tiles(plan):
-        assert n >= 1 and (name < 0 or n <= rows) and n <= 64
+    for i, (name, start, n, _) in enumerate(plan.tiles):
+        assert 1 <= n <= 64 and (name < 0) == (i >= plan.n_tiles) and (name < 0 or n <= plan.tile_rows)
         seen += range(start, start + n)
         assert all(max(ids[order[p]], -1) == name for p in range(start, start + n))
     assert sorted(seen) == list(range(len(ids)))
