@@ -66,7 +66,10 @@ __device__ __forceinline__ uint4 ad_zero() { return make_uint4(0u, 0u, 0u, 0u); 
 // h rows of 16-bit values: 8 more than the rank, so that the rows of a fragment lie in different banks
 __host__ __device__ constexpr int ad_pitch(int rank) { return (rank + 15) / 16 * 16 + 8; }
 
-__device__ __forceinline__ const uint16_t* ad_row(const void* p, int row, int ld) { return reinterpret_cast<const uint16_t*>(p) + static_cast<int64_t>(row) * ld; }
+// (ld: values between rows, below 2^30)
+__device__ __forceinline__ const uint16_t* ad_row(const void* p, int row, int ld) {
+    return reinterpret_cast<const uint16_t*>(reinterpret_cast<const char*>(p) + static_cast<int64_t>(row) * (ld * 2));
+}
 
 // acc = 16 rows of x times NT * 8 rows of down (those from rb on), over the columns k0 to k1 in blocks of 32, of which this warp has number `b` and
 // every `step`-th after it. U of them are asked for at once: with fewer on the way the sum waits for memory (4099 rows x 4096, rank 32: 31.8 us
@@ -116,9 +119,8 @@ __device__ __forceinline__ void ad_down(float (&acc)[NT][4], const uint16_t* x0,
 
 // one row's largest |h| -> the power of two that brings it to 2^8 ... 2^9, and that power's reciprocal, both normal numbers
 __device__ __forceinline__ float2 ad_row_scale(float m) {
-    int e = 9;
-    if (m > 0.0f && m < INFINITY) frexpf(m, &e);
-    e = min(max(e - 9, -126), 126);
+    const int b = static_cast<int>(__float_as_uint(m) >> 23);               // exponent + 127
+    const int e = b == 255 || m == 0.0f ? 0 : min(max(b - 127 - 8, -126), 126);
     return make_float2(__uint_as_float(static_cast<uint32_t>(127 - e) << 23), __uint_as_float(static_cast<uint32_t>(127 + e) << 23));
 }
 template <bool kBf16>
@@ -162,6 +164,9 @@ __device__ __forceinline__ void ad_copy(const AdapterArgs& a, const int4& tile, 
     }
 }
 
+// (RANK: of these kernels, or 0 where it is only known when they run: with it addresses are constants and no step is half empty. 64 rows with 61
+// adapters, rank 16, 4096 -> 11008: 13.2 us without, 10.7 with it.)
+
 // ---- few rows --------------------------------------------------------------------------------------------------------------
 // Each warp has a ring of its own for its groups of 32 rows of `up` (contiguous: one bulk copy each), filled from the start on: 4 groups up to rank
 // 16, 2 beyond. Longer rows than 64 values have no room, and go from memory to registers.
@@ -176,13 +181,13 @@ __host__ __device__ constexpr size_t ad_few_smem_bytes(int rank) {
            static_cast<size_t>(2) * 16 * ad_pitch(rank) * 2;
 }
 
-template <int NT, bool kBf16>
+template <int NT, int RANK, bool kBf16>
 __global__ void __launch_bounds__(kAdThreads, 2) adapter_few_kernel(const AdapterArgs a) {
     constexpr int C = NT * 8;
     extern __shared__ __align__(16) uint8_t ad_smem[];
     __shared__ float row_scale[16];
     __shared__ uint64_t full[kAdWarps][4];
-    const int rank = a.rank, padded = (rank + C - 1) / C * C, pitch = ad_pitch(rank), slots = ad_ring_slots(rank), ctas = a.cluster;
+    const int rank = RANK > 0 ? RANK : a.rank, padded = (rank + C - 1) / C * C, pitch = ad_pitch(rank), slots = ad_ring_slots(rank), ctas = a.cluster;
     float* red = reinterpret_cast<float*>(ad_smem + kAdWarps * ad_ring_bytes(rank));      // [8 warps][16][C]
     float* part = red + kAdWarps * 16 * C;                            // [8 CTAs][16][C]
     float* h = part + kAdCluster * 16 * C;                            // [16][padded]
@@ -329,30 +334,90 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_few_kernel(const Adapte
 // tiles of 16 rows that a tile of so many rows has: 1, 2 or 4, so that they divide the warps
 __device__ __forceinline__ int ad_m_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
+__device__ __forceinline__ void ad_copy_async(uint32_t dst, const void* src, bool in) {      // 16 bytes, or zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ad_copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void ad_copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// A stage holds 64 rows and columns of x (64 x 64, 32 x 128 or 16 x 256 values: 8 KB) and the same columns of NT * 8 rows of down. Every second row
+// has the halves of its 128 bytes exchanged, so that the eight 16-byte pieces that a quarter of a warp reads, four of each of two rows, lie in
+// different banks.
+template <int NT>
+__host__ __device__ constexpr int ad_stage_bytes(int m_tiles) { return 8192 + NT * 8 * 512 / m_tiles; }
+template <int NT>
+__host__ __device__ constexpr int ad_stages(int m_tiles) { return NT == 8 && m_tiles == 1 ? 2 : 4; }     // two CTAs per SM have room
+template <int NT>
+__host__ __device__ constexpr int ad_down_smem_bytes() { return NT == 8 ? 4 * ad_stage_bytes<NT>(2) : 4 * ad_stage_bytes<NT>(1); }
+
 template <int NT, bool kBf16>
 __global__ void __launch_bounds__(kAdThreads, 2) adapter_down_kernel(const AdapterArgs a) {
     constexpr int C = NT * 8;
-    __shared__ __align__(16) float red[kAdWarps][16][C];
+    extern __shared__ __align__(16) uint8_t ad_smem[];
+    float* red = reinterpret_cast<float*>(ad_smem);       // [8 warps][16][C], when the stages have been read
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int4 tile = a.tiles[blockIdx.x];
     const int32_t* rows = a.tile_rows + blockIdx.x * kAdRows;
     const int m_tiles = ad_m_tiles(tile.z), mt = warp % m_tiles, kw = warp / m_tiles, k_warps = kAdWarps / m_tiles;
-    const uint16_t *x0 = ad_row(a.x, rows[mt * 16 + g], a.ld_x), *x1 = ad_row(a.x, rows[mt * 16 + g + 8], a.ld_x);
+    const int pieces = 32 / m_tiles, columns = pieces * 8;              // 16-byte pieces and values of a row in a stage
+    const int p_log2 = m_tiles == 1 ? 5 : m_tiles == 2 ? 4 : 3;
+    const uint16_t* x[2];                                               // my piece of two rows of x per stage
+    const int piece = tid & (pieces - 1), first = tid >> p_log2, apart = kAdThreads >> p_log2;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = ad_row(a.x, rows[first + i * apart], a.ld_x);
     // (in this order: the second kernel, which may start from here on, reads what came before this one without a wait)
     griddep_wait();
     griddep_launch_dependents();
     if (tile.x < 0 || tile.x >= a.n_adapters) return;
-    const int k0 = blockIdx.y * a.k_part, k1 = min(a.width, k0 + a.k_part);
+    const int k0 = blockIdx.y * a.k_part, k1 = min(a.width, k0 + a.k_part), n_stages = (k1 - k0 + columns - 1) / columns;
     const uint16_t* down = reinterpret_cast<const uint16_t*>(a.down) + static_cast<int64_t>(tile.x) * a.rank * a.width;
     float* h = a.h + (static_cast<int64_t>(blockIdx.y) * a.rows + tile.y) * a.rank;
+    const int stage_bytes = ad_stage_bytes<NT>(m_tiles), stages = ad_stages<NT>(m_tiles);
+    const uint32_t smem = smem_u32(ad_smem);
+    auto place = [&](int row, int p) { return static_cast<uint32_t>((row << p_log2) + (p ^ (row & 1) << 2)) * 16u; };
     for (int rb = 0; rb < a.rank; rb += C) {
+        auto load = [&](int s) {        // (always ends a group, an empty one behind the last stage)
+            if (s < n_stages) {
+                const uint32_t to = smem + (s & (stages - 1)) * stage_bytes;
+                const int k = k0 + s * columns + piece * 8;
+                const bool in = k < k1;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) ad_copy_async(to + place(first + i * apart, piece), x[i] + (in ? k : k0), in);
+                for (int r = first; r < C; r += apart)
+                    ad_copy_async(to + 8192 + place(r, piece), down + static_cast<int64_t>(min(rb + r, a.rank - 1)) * a.width + (in ? k : k0), in);
+            }
+            ad_copies_end();
+        };
         float acc[NT][4];
-        ad_down<NT, kBf16, NT == 8 ? 2 : NT == 4 ? 3 : 4>(acc, x0, x1, down, rb, a.rank, a.width, k0, k1, kw, k_warps, g, t);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
         if (rb > 0) __syncthreads();
+        for (int s = 0; s < stages - 1; ++s) load(s);
+        for (int s = 0; s < n_stages; ++s) {
+            if (stages == 4) ad_copies_wait<2>();
+            else ad_copies_wait<0>();
+            __syncthreads();             // stage s is there, and stage s - 1 has been read
+            load(s + stages - 1);
+            const uint8_t* from = ad_smem + (s & (stages - 1)) * stage_bytes;
+            // blocks of 32 columns: one of this warp's per stage
+            const int p = kw * 4 + t;
+            const uint4 xa = *reinterpret_cast<const uint4*>(from + place(mt * 16 + g, p)), xb = *reinterpret_cast<const uint4*>(from + place(mt * 16 + g + 8, p));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const uint4 d = *reinterpret_cast<const uint4*>(from + 8192 + place(j * 8 + g, p));
+                mma_m16n8k16<kBf16>(acc[j], xa.x, xb.x, xa.y, xb.y, d.x, d.y);
+                mma_m16n8k16<kBf16>(acc[j], xa.z, xb.z, xa.w, xb.w, d.z, d.w);
+            }
+        }
+        ad_copies_wait<0>();
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            *reinterpret_cast<float2*>(&red[warp][g][j * 8 + 2 * t]) = make_float2(acc[j][0], acc[j][1]);
-            *reinterpret_cast<float2*>(&red[warp][g + 8][j * 8 + 2 * t]) = make_float2(acc[j][2], acc[j][3]);
+            *reinterpret_cast<float2*>(red + (warp * 16 + g) * C + j * 8 + 2 * t) = make_float2(acc[j][0], acc[j][1]);
+            *reinterpret_cast<float2*>(red + (warp * 16 + g + 8) * C + j * 8 + 2 * t) = make_float2(acc[j][2], acc[j][3]);
         }
         __syncthreads();
         for (int i = tid; i < tile.z * C / 4; i += kAdThreads) {
@@ -360,7 +425,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_down_kernel(const Adapt
             if (rb + c >= a.rank) continue;
             float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             for (int w = 0; w < k_warps; ++w) {
-                const float4 v = *reinterpret_cast<const float4*>(&red[w * m_tiles + (r >> 4)][r & 15][c]);
+                const float4 v = *reinterpret_cast<const float4*>(red + ((w * m_tiles + (r >> 4)) * 16 + (r & 15)) * C + c);
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
             *reinterpret_cast<float4*>(h + static_cast<int64_t>(r) * a.rank + rb + c) = s;
@@ -368,22 +433,25 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_down_kernel(const Adapt
     }
 }
 
-// KS: k-steps of 16 whose part of `up` a warp has in registers at once. CTA y of a tile has the groups of 256 outputs y, y + gridDim.y, ...
-template <int KS, bool kBf16>
+// CTA y of a tile has the groups of 256 outputs y, y + gridDim.y, ..., a warp 32 of each. Base goes through a ring in shared memory, all stages of
+// which are asked for before h is waited for; `up` goes to registers, KS k-steps of 16 of the next group while this one is computed.
+__host__ __device__ constexpr int ad_base_stages(int rank) { return rank <= 32 ? 3 : 2; }      // so that two CTAs fit an SM up to rank 64
+__host__ __device__ constexpr int ad_up_smem_bytes(int rank) { return ad_base_stages(rank) * kAdRows * kAdCols * 2 + 2 * kAdRows * ad_pitch(rank) * 2; }
+
+template <int KS, int RANK, bool kBf16>
 __global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const AdapterArgs a) {
     extern __shared__ __align__(16) uint8_t ad_smem[];
     __shared__ float row_scale[kAdRows];
     __shared__ int rows[kAdRows];
-    const int rank = a.rank, pitch = ad_pitch(rank), k_steps = (rank + 15) / 16;
-    uint16_t* h_hi = reinterpret_cast<uint16_t*>(ad_smem);            // [64][pitch]
+    const int rank = RANK > 0 ? RANK : a.rank, pitch = ad_pitch(rank), k_steps = (rank + 15) / 16, stages = ad_base_stages(rank);
+    uint16_t* h_hi = reinterpret_cast<uint16_t*>(ad_smem + stages * kAdRows * kAdCols * 2);            // [64][pitch]
     uint16_t* h_lo = h_hi + kAdRows * pitch;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int4 tile = a.tiles[blockIdx.x];
-    const int n_step = gridDim.y * kAdCols;
-    int n = blockIdx.y * kAdCols + warp * 32;
+    const int n_step = gridDim.y * kAdCols, n_first = blockIdx.y * kAdCols;
     if (tile.x < 0 || tile.x >= a.n_adapters) {
         pdl_enter();
-        for (int c = blockIdx.y * kAdCols; c < a.outputs; c += n_step) ad_copy(a, tile, a.tile_rows + blockIdx.x * kAdRows, c, min(a.outputs, c + kAdCols));
+        for (int c = n_first; c < a.outputs; c += n_step) ad_copy(a, tile, a.tile_rows + blockIdx.x * kAdRows, c, min(a.outputs, c + kAdCols));
         return;
     }
     // ---- what does not need h: all of it was there before the first kernel let this one start ----
@@ -391,70 +459,83 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const Adapter
     const uint16_t* up = reinterpret_cast<const uint16_t*>(a.up) + static_cast<int64_t>(tile.x) * a.outputs * rank;
     if (tid < kAdRows) rows[tid] = a.tile_rows[blockIdx.x * kAdRows + tid];
     const float scale = a.scales[tile.x];
-    uint2 u[KS][4];
-    uint4 base[kAdRows / 16][2];
     const int first = (g >> 1) * 8 + (g & 1);                 // my row of `up` in a group of 32
     const uint16_t* my_up = up + static_cast<int64_t>(first) * rank + t * 4;
-    auto ask = [&](int at) {        // the first k-steps of `up` and all of base, for the 32 outputs from `at` on
+    uint2 next[KS][4];
+    auto ask = [&](int at) {        // the first k-steps of `up` for the 32 outputs from `at` on
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) ad_up_load(u[ks], my_up + static_cast<int64_t>(at) * rank + ks * 16, rank, a.outputs - at - first, ks * 16 + t * 4 < rank);
-        if (at + t * 8 < a.outputs) {
-#pragma unroll
-            for (int m = 0; m < kAdRows / 16; ++m)
-                if (m < m_tiles) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) base[m][e] = *reinterpret_cast<const uint4*>(ad_row(a.base, rows[m * 16 + g + 8 * e], a.ld_base) + at + t * 8);
-                }
-        }
+        for (int ks = 0; ks < KS; ++ks) ad_up_load(next[ks], my_up + static_cast<int64_t>(at) * rank + ks * 16, rank, a.outputs - at - first, ks * 16 + t * 4 < rank);
     };
     __syncthreads();
-    ask(n);
+    // a stage: 16 rows per m-tile of 512 bytes; a warp copies a row at a time
+    const uint32_t smem = smem_u32(ad_smem);
+    auto load = [&](int i) {        // base of group number i (always ends a group of copies, an empty one behind the last)
+        const int n = n_first + i * n_step + lane * 8;
+        if (n < a.outputs) {
+            const uint32_t to = smem + i % stages * (kAdRows * kAdCols * 2) + lane * 16;
+            for (int r = warp; r < min(m_tiles * 16, tile.z); r += kAdWarps) ad_copy_async(to + r * kAdCols * 2, ad_row(a.base, rows[r], a.ld_base) + n, true);
+        }
+        ad_copies_end();
+    };
+    for (int i = 0; i < stages; ++i) load(i);
+    ask(n_first + warp * 32);
     griddep_wait();
     griddep_launch_dependents();
-    // ---- h, summed over the parts of the width: four values per thread, a row's in neighbouring ones (of a power of two of lanes) ----
+    // ---- h, summed over the parts of the width, in two 16-bit values: a row has a power of two of lanes, four values each at a time ----
     const float* h = a.h + static_cast<int64_t>(tile.y) * rank;
     const int64_t part = static_cast<int64_t>(a.rows) * rank;
-    const int quads = k_steps * 4;                                     // of a row, the last two behind an odd rank / 8
-    if constexpr (kBf16) {
-        for (int i = tid; i < m_tiles * 16 * quads; i += kAdThreads) {
-            const int r = i / quads, c = i % quads * 4;
-            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int lanes = rank <= 16 ? 4 : rank <= 32 ? 8 : rank <= 64 ? 16 : 32, per_warp = 32 / lanes, c0 = (lane & (lanes - 1)) * 4;
+    for (int r = warp * per_warp + lane / lanes; r < m_tiles * 16; r += kAdWarps * per_warp) {
+        float4 s[kAdMaxRank / 128];
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kAdMaxRank / 128; ++i) {
+            s[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int c = c0 + i * 128;
             if (r < tile.z && c < rank)
                 for (int p = 0; p < a.k_parts; ++p) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(h + p * part + static_cast<int64_t>(r) * rank + c));
-                    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(h + p * part + r * rank + c));
+                    s[i].x += v.x; s[i].y += v.y; s[i].z += v.z; s[i].w += v.w;
                 }
-            const uint32_t h0 = pack2<true>(s.x, s.y), h1 = pack2<true>(s.z, s.w);
-            auto rest = [](float v, float hi) { const float d = v - hi; return fabsf(d) < INFINITY ? d : 0.0f; };
-            *reinterpret_cast<uint2*>(h_hi + r * pitch + c) = make_uint2(h0, h1);
-            *reinterpret_cast<uint2*>(h_lo + r * pitch + c) = make_uint2(pack2<true>(rest(s.x, bf16_lo(h0)), rest(s.y, bf16_hi(h0))),
-                                                                         pack2<true>(rest(s.z, bf16_lo(h1)), rest(s.w, bf16_hi(h1))));
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(s[i].x), fabsf(s[i].y)), fmaxf(fabsf(s[i].z), fabsf(s[i].w))));
         }
-    } else {          // a warp has whole rows, for their largest values
-        for (int r = warp; r < m_tiles * 16; r += kAdWarps) {
-            float v[kAdMaxRank / 32], m = 0.0f;
+        float2 f = make_float2(1.0f, 1.0f);
+        if constexpr (!kBf16) {
+            for (int o = lanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            f = ad_row_scale(m);
+            if (c0 == 0) row_scale[r] = f.y;
+        }
 #pragma unroll
-            for (int i = 0; i < kAdMaxRank / 32; ++i) {
-                const int c = i * 32 + lane;
-                v[i] = 0.0f;
-                if (i * 32 >= rank) break;
-                if (r < tile.z && c < rank)
-                    for (int p = 0; p < a.k_parts; ++p) v[i] += __ldcg(h + p * part + static_cast<int64_t>(r) * rank + c);
-                m = fmaxf(m, fabsf(v[i]));
-            }
-            const float2 f = ad_row_scale(warp_max(m));
-            if (lane == 0) row_scale[r] = f.y;
-#pragma unroll
-            for (int i = 0; i < kAdMaxRank / 32; ++i) {
-                const int c = i * 32 + lane;
-                if (i * 32 >= k_steps * 16) break;
-                if (c < k_steps * 16) ad_split<kBf16>(v[i] * f.x, h_hi[r * pitch + c], h_lo[r * pitch + c]);
-            }
+        for (int i = 0; i < kAdMaxRank / 128; ++i) {
+            const int c = c0 + i * 128;
+            if (c >= k_steps * 16) continue;
+            s[i].x *= f.x; s[i].y *= f.x; s[i].z *= f.x; s[i].w *= f.x;
+            const uint2 hi = make_uint2(pack2<kBf16>(s[i].x, s[i].y), pack2<kBf16>(s[i].z, s[i].w));
+            auto rest = [](float v, float of) { const float d = v - of; return fabsf(d) < INFINITY ? d : 0.0f; };
+            *reinterpret_cast<uint2*>(h_hi + r * pitch + c) = hi;
+            *reinterpret_cast<uint2*>(h_lo + r * pitch + c) =
+                make_uint2(pack2<kBf16>(rest(s[i].x, unpack_lo<kBf16>(hi.x)), rest(s[i].y, unpack_hi<kBf16>(hi.x))),
+                           pack2<kBf16>(rest(s[i].z, unpack_lo<kBf16>(hi.y)), rest(s[i].w, unpack_hi<kBf16>(hi.y))));
         }
     }
-    __syncthreads();
-    for (; n - warp * 32 < a.outputs; n += n_step) {       // (a warp whose 32 are behind the end asks for nothing and writes nothing)
-        const int col = n + t * 8;
+    int row[kAdRows / 16][2];
+#pragma unroll
+    for (int m = 0; m < kAdRows / 16; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) row[m][e] = rows[m * 16 + g + 8 * e];
+    for (int i = 0, n0 = n_first; n0 < a.outputs; ++i, n0 += n_step) {
+        const int n = n0 + warp * 32, col = n + t * 8;        // (a warp whose 32 are behind the end writes nothing)
+        uint2 u[KS][4];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) u[ks][q] = next[ks][q];
+        ask(n + n_step);
+        if (stages == 3) ad_copies_wait<2>();
+        else ad_copies_wait<1>();
+        __syncthreads();            // the stage is there, and h
+        uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + col;
+        const uint8_t* base = ad_smem + i % stages * (kAdRows * kAdCols * 2) + (warp * 32 + t * 8) * 2;
 #pragma unroll
         for (int m = 0; m < kAdRows / 16; ++m) {
             if (m >= m_tiles) break;
@@ -471,16 +552,18 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const Adapter
 #pragma unroll
             for (int e = 0; e < 2; ++e)
                 if (col < a.outputs && r0 + 8 * e < tile.z)
-                    *reinterpret_cast<uint4*>(const_cast<uint16_t*>(ad_row(a.out, rows[r0 + 8 * e], a.ld_out)) + col) =
-                        ad_join<kBf16>(base[m][e], acc, 2 * e, kBf16 ? scale : scale * row_scale[r0 + 8 * e]);
+                    *reinterpret_cast<uint4*>(const_cast<uint16_t*>(ad_row(out, row[m][e], a.ld_out))) =
+                        ad_join<kBf16>(*reinterpret_cast<const uint4*>(base + (r0 + 8 * e) * kAdCols * 2), acc, 2 * e, kBf16 ? scale : scale * row_scale[r0 + 8 * e]);
         }
-        ask(n + n_step);
+        __syncthreads();            // the stage has been read
+        load(i + stages);
     }
+    ad_copies_wait<0>();
 }
 
-template <int NT, bool kBf16>
+template <int NT, int RANK, bool kBf16>
 static int launch_few(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
-    auto kern = adapter_few_kernel<NT, kBf16>;
+    auto kern = adapter_few_kernel<NT, RANK, kBf16>;
     static bool configured[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -495,18 +578,19 @@ static int launch_few(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
     return HDS_OK;
 }
 
-template <int NT, int KS, bool kBf16>
+template <int NT, int KS, int RANK, bool kBf16>
 static int launch_many(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
-    auto up = adapter_up_kernel<KS, kBf16>;
-    const size_t smem = static_cast<size_t>(2) * kAdRows * ad_pitch(a.rank) * 2;
+    auto down = adapter_down_kernel<NT, kBf16>;
+    auto up = adapter_up_kernel<KS, RANK, kBf16>;
     static bool configured[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        HDS_CHECK_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kAdRows * ad_pitch(kAdMaxRank) * 2));
+        HDS_CHECK_CUDA(cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, ad_down_smem_bytes<NT>()));
+        HDS_CHECK_CUDA(cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, ad_up_smem_bytes(KS == 1 ? 16 : KS == 2 ? 32 : kAdMaxRank)));
         configured[dev & 63] = true;
     }
-    HDS_CHECK_CUDA(launch_kernel(adapter_down_kernel<NT, kBf16>, dim3(n_tiles, a.k_parts), dim3(kAdThreads), 0, s, a));
+    HDS_CHECK_CUDA(launch_kernel(down, dim3(n_tiles, a.k_parts), dim3(kAdThreads), ad_down_smem_bytes<NT>(), s, a));
     // CTAs of a tile: the fewest waves of two per SM, a CTA's beginning and end counted as one group of outputs
     const int groups = (a.outputs + kAdCols - 1) / kAdCols, slots = 2 * sm_count();
     int parts = 1;
@@ -519,27 +603,34 @@ static int launch_many(const AdapterArgs& a, int n_tiles, cudaStream_t s) {
         }
         if (static_cast<int64_t>(n_tiles) * p >= slots && p >= 8) break;
     }
-    HDS_CHECK_CUDA(launch_kernel(up, dim3(n_tiles, parts), dim3(kAdThreads), smem, s, a));
+    HDS_CHECK_CUDA(launch_kernel(up, dim3(n_tiles, parts), dim3(kAdThreads), ad_up_smem_bytes(a.rank), s, a));
     return HDS_OK;
 }
 
+template <int NT, int RANK, bool kBf16>
+static int launch_adapters_as(const AdapterArgs& a, int n_tiles, bool few, cudaStream_t s) {
+    return few ? launch_few<NT, RANK, kBf16>(a, n_tiles, s) : launch_many<NT, NT / 2, RANK, kBf16>(a, n_tiles, s);
+}
 template <bool kBf16>
 static int launch_adapters(const AdapterArgs& a, int n_tiles, bool few, cudaStream_t s) {
-    if (few)
-        return a.rank <= 16 ? launch_few<2, kBf16>(a, n_tiles, s) : a.rank <= 32 ? launch_few<4, kBf16>(a, n_tiles, s) : launch_few<8, kBf16>(a, n_tiles, s);
-    return a.rank <= 16 ? launch_many<2, 1, kBf16>(a, n_tiles, s) : a.rank <= 32 ? launch_many<4, 2, kBf16>(a, n_tiles, s) : launch_many<8, 4, kBf16>(a, n_tiles, s);
+    if (a.rank == 16) return launch_adapters_as<2, 16, kBf16>(a, n_tiles, few, s);
+    if (a.rank == 32) return launch_adapters_as<4, 32, kBf16>(a, n_tiles, few, s);
+    if (a.rank == 64) return launch_adapters_as<8, 64, kBf16>(a, n_tiles, few, s);
+    return a.rank < 16 ? launch_adapters_as<2, 0, kBf16>(a, n_tiles, few, s)
+           : a.rank < 32 ? launch_adapters_as<4, 0, kBf16>(a, n_tiles, few, s) : launch_adapters_as<8, 0, kBf16>(a, n_tiles, few, s);
 }
 
 }  // namespace hds
 
 using namespace hds;
 
-// Parts of the width of the first of two kernels: two CTAs on every SM, of at least 256 columns each.
+// Parts of the width of the first of two kernels: two CTAs on every SM, of at least 256 columns each, and no more than 16, which the second one adds
+// up (215 rows of 9 adapters, rank 64, 8192 -> 8192: 12.2 us with 16, 12.5 with 32, 14.4 with 8).
 extern "C" int hds_adapter_parts(int n_tiles, int width) {
     const int most = (width + 255) / 256;
     int parts = n_tiles > 0 ? (2 * sm_count() + n_tiles / 2) / n_tiles : 1;
     parts = parts < 1 ? 1 : parts > most ? most : parts;
-    return parts > 32 ? 32 : parts;
+    return parts > 16 ? 16 : parts;
 }
 
 extern "C" int hds_adapter_add(const void* base, int64_t ld_base, const void* x, int64_t ld_x, const void* down, const void* up, const float* scales,
@@ -565,7 +656,7 @@ extern "C" int hds_adapter_add(const void* base, int64_t ld_base, const void* x,
     a.n_adapters = n_adapters; a.rank = rank; a.width = width; a.outputs = outputs; a.rows = rows;
     const bool few = workspace == nullptr;
     HDS_REQUIRE(!few || most_rows <= kAdFew, "adapter_add: tiles of more than 16 rows need a workspace");
-    a.cluster = getenv("HDS_ADC") ? atoi(getenv("HDS_ADC")) : n_tiles * 8 <= sm_count() ? 8 : 4;
+    a.cluster = n_tiles * 8 <= sm_count() ? 8 : 4;
     if (!few) {
         const int parts = hds_adapter_parts(n_tiles, width);
         a.k_part = ((width + parts - 1) / parts + 31) / 32 * 32;

@@ -973,8 +973,6 @@ def retention_stuck() -> bool:
 # (A step makes hundreds of these calls: their checks read each attribute once, and a stream is asked for by its number. A Stream object and
 # a device guard alone cost 5 us of the 22 that a call took; it takes 9 to 12 so.)
 _raw_stream = torch._C._cuda_getCurrentRawStream
-import os
-_ADAPTER_TWO = int(os.environ.get('HDS_ADTWO', '0'))
 
 
 def _place(t: torch.Tensor, name: str) -> int:
@@ -1050,7 +1048,7 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
     lib = native.cuda_lib()
     with _On(index):
         ws, n_bytes = None, 0
-        if plan.tile_rows > ADAPTER_FEW or _ADAPTER_TWO:
+        if plan.tile_rows > ADAPTER_FEW:
             n_bytes = lib.hds_adapter_parts(count, K) * T * R * 4
             ws = x.new_empty(n_bytes // 2)       # of this call alone: a plan may be in use on several streams, and in graphs
         rc = lib.hds_adapter_add(p_base, ld_base, x.data_ptr(), ld_x, down.data_ptr(), up.data_ptr(), scales.data_ptr(), n, R, K, N, T,
