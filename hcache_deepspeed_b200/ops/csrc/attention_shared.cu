@@ -2,14 +2,16 @@
 //
 //   softmax over prefix and own keys = the two parts' (m, l, O) joined:  O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i
 //
-// 1. Prefix. All query rows of a group of sequences, (token, query head of the KV head's group) pairs, are rows of one matrix product:
-//    a CTA has 128 of them, one KV head and a part of the prefix, in tiles of 128 keys:
-//      warp 0    : TMA producer - Q once (one 3-D box: tokens x heads x 64 dims), then K / V tiles page by page (2-stage ring, SWIZZLE_128B);
-//                  what is behind the prefix in its last tile comes from behind the cache, that is, as zeros
-//      warp 1    : TMEM allocator, tcgen05.mma issuer: S = Q K^T, O += P V (V MN-major, as its pages have it)
-//      warps 2-9 : softmax - two threads per row, 64 key columns each, row maxima exchanged through shared memory; P goes to shared memory in
-//                  16 bits. O stays in TMEM and is rescaled only when a row's maximum grows by more than 2^8.
-//    No causal edge: every row comes behind the whole prefix. (m, l, O) in fp32 go to scratch, one part per split.
+// 1. Prefix. All query rows of a group of sequences, (token, query head of the KV head's group) pairs, are rows of one matrix product. A CTA has
+//    one KV head, a part of the prefix in tiles of 128 keys, and up to 256 rows: two streams of 128, so that the products of one run while the
+//    other one's scores are weighed (the scheme of attention_pair.cuh). With more than 128 rows the streams are two row tiles that see the
+//    same keys; with fewer they share the rows and take the key tiles in turn, as two more parts of the prefix.
+//      warp 0    : TMA producer - Q (3-D boxes: tokens x heads x 64 dims), then K and V tiles page by page in the order of their use, through one
+//                  ring; what is behind the prefix in its last tile comes from behind the cache, that is, as zeros
+//      warp 1    : TMEM allocator, tcgen05.mma issuer: O += P V, then S = Q K^T of the stream's next tile (V MN-major, as its pages have it)
+//      warps 2-9 : softmax, four warps per stream, one thread per row; P goes back to TMEM as 16-bit pairs, over the scores it came from. O stays in
+//                  TMEM and is rescaled only when a row's maximum grows by more than 2^8
+//    No causal edge: every row comes behind the whole prefix. (m, l, O) in fp32 go to scratch, one part per split and key stream.
 // 2. Own keys, and the end. A CTA has up to 8 query rows of a sequence and KV head; its warps take strips of 16 keys through rings of their
 //    own (TMA, three strips ahead, see attention_group.cu, whose arithmetic this is: mma.sync, the weights' rounding kept in the
 //    MMA's other 8 rows). Splits of a long sequence are a cluster and meet in its shared memory; there the prefix' parts join, and the rows are
@@ -27,9 +29,8 @@
 
 namespace hds {
 
-constexpr int kSpThreads = 320;   // TMA warp + MMA warp + 8 softmax warps
-constexpr int kSpTok = 128;
-constexpr int kSpStages = 2;
+constexpr int kSpThreads = 320;   // TMA warp + MMA warp + 2 x 4 softmax warps
+constexpr int kSpTok = 128;       // keys of a tile, rows of a stream
 constexpr int kOwnRows = 8;       // query rows of a CTA of the second part
 constexpr int kOwnStrip = 16;     // keys a warp takes at a time; pages hold a multiple
 constexpr int kOwnWarps = 4;
@@ -40,14 +41,15 @@ struct SharedArgs {
     int64_t ld_q, ld_out;
     const int32_t* block_tables;
     int max_blocks_per_seq;
-    const int4* tiles;      // prefix: (sequence whose table names the pages, first query row, tokens, prefix length)
+    const int4* tiles;      // prefix: (sequence whose table names the pages, first query row, tokens of up to two streams, prefix length)
     const int4* items;      // own keys: pairs (sequence, first query row, tokens, keys), (prefix length, 0, 0, 0)
     int rows, n_q_heads, n_kv_heads, block_size, bs_log2, num_rows_kv;
-    int tile_tokens;        // tokens of a full tile
+    int tile_tokens;        // tokens of a stream of rows
     int p_splits, row_tiles;
+    int has_prefix;         // the first kernel runs
     float scale_log2;
-    float* ws_ml;           // [p_splits][rows][n_q_heads][2]
-    float* ws_o;            // [p_splits][rows][n_q_heads][D]
+    float* ws_ml;           // [2 p_splits][rows][n_q_heads][2]; m = -inf: nothing in ws_o
+    float* ws_o;            // [2 p_splits][rows][n_q_heads][D]
 };
 
 __device__ __forceinline__ float sp_ex2(float x) {
@@ -55,12 +57,25 @@ __device__ __forceinline__ float sp_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// splits of a prefix that have tiles, and tiles of each
-__host__ __device__ inline int sp_tiles_per_split(int prefix, int splits) { return ((prefix + kSpTok - 1) / kSpTok + splits - 1) / splits; }
+// tiles of 16-bit values in shared memory: Q's one or two, the others a ring of K and V
+__host__ __device__ constexpr int sp_tiles(int d) { return d == 128 ? 7 : 13; }
+__host__ __device__ constexpr size_t sp_smem_bytes(int d) { return static_cast<size_t>(sp_tiles(d)) * kSpTok * d * 2 + 512 + 1024; }
 
-template <int D>
-__host__ __device__ constexpr size_t sp_smem_bytes() {
-    return static_cast<size_t>(128) * D * 2 + 128 * 128 * 2 + static_cast<size_t>(kSpStages) * 2 * kSpTok * D * 2 + 256 + 2 * 2 * 128 * 4 + 1024;
+__device__ __forceinline__ uint64_t sp_pack(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void sp_unpack(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t sp_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t sp_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 template <int D, bool kBf16>
@@ -69,271 +84,285 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     constexpr int PANELS = D / 64;
     constexpr int PANEL_BYTES = kSpTok * 128;
     constexpr int TILE_BYTES = PANELS * PANEL_BYTES;
-    constexpr uint32_t TMEM_COLS = 256;
+    constexpr int MAX_SLOTS = sp_tiles(D) - 1;
     constexpr uint32_t IDESC_QK = make_idesc_f16(128, kSpTok, kBf16, false, false);
     constexpr uint32_t IDESC_PV = make_idesc_f16(128, D, kBf16, false, true);
     constexpr float kUpLog2 = kBf16 ? 0.0f : 7.0f;     // (2^8 of a stale maximum and these stay below fp16's 2^16)
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* q_sm = smem;
-    uint8_t* p_sm = q_sm + TILE_BYTES;
-    uint8_t* kv_sm = p_sm + 2 * PANEL_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(kv_sm + kSpStages * 2 * TILE_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sp_tiles(D) * TILE_BYTES);
     uint64_t* q_full = bars;
-    uint64_t* kv_full = bars + 1;
-    uint64_t* kv_empty = kv_full + kSpStages;
-    uint64_t* s_full = kv_empty + kSpStages;
-    uint64_t* p_full = s_full + 1;
-    uint64_t* o_full = p_full + 1;
-    uint64_t* s_empty = o_full + 1;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_empty + 1);
-    float* xch = reinterpret_cast<float*>(tmem_slot + 2);
+    uint64_t* full = bars + 1;
+    uint64_t* empty = full + MAX_SLOTS;
+    uint64_t* s_full = empty + MAX_SLOTS;    // [stream] S of a tile is there (and P V of the tile before is done)
+    uint64_t* p_full = s_full + 2;           // [stream] P is there (and O rescaled)
+    uint64_t* o_full = p_full + 2;           // [stream] the last P V is done
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+    static_assert((1 + 2 * MAX_SLOTS + 6) * 8 + 4 <= 512, "barriers have room");
 
     const uint32_t warp = warp_id(), lane = lane_id();
-    pdl_enter();
-    const int4 tile = a.tiles[blockIdx.x];
+    const int4 tile = a.tiles[blockIdx.x];      // (the plan: no kernel writes it)
+    // (in this order: the second kernel, which may start from here on, reads what came before this one without a wait)
+    griddep_wait();
+    griddep_launch_dependents();
     const int kvh = blockIdx.y, split = blockIdx.z;
     const int G = a.n_q_heads / a.n_kv_heads;
-    const int n_live_rows = tile.z * G;
+    const bool two = tile.z > a.tile_tokens;    // two row tiles; else one, whose key tiles the streams share
     const int prefix = tile.w;
     const int tiles_total = (prefix + kSpTok - 1) / kSpTok;
-    const int tps = sp_tiles_per_split(prefix, a.p_splits);
-    const int t0 = split * tps;
-    if (t0 >= tiles_total) return;
-    const int n_tiles = min(tiles_total, t0 + tps) - t0;
-    const int bs = a.block_size;
-    const int bps = kSpTok / bs;
+    const int t0 = static_cast<int>(static_cast<int64_t>(tiles_total) * split / a.p_splits);
+    const int n_tiles = static_cast<int>(static_cast<int64_t>(tiles_total) * (split + 1) / a.p_splits) - t0;
+    const int slots = sp_tiles(D) - (two ? 2 : 1);
+    uint8_t* q_sm = smem;                       // [row tile][panel][128 x 64]
+    uint8_t* ring = smem + (two ? 2 : 1) * TILE_BYTES;
+    const int bs = a.block_size, bps = kSpTok / bs;
+    // places of K and V of a key tile in the producer's order: K0 K1 V0 K2 V1 ... (two row tiles: K1 is asked for behind K0's products only)
+    auto seq_k = [&](int t) { return t < 2 ? t : 2 * t - 1; };
+    auto seq_v = [&](int t) { return n_tiles == 1 ? 1 : t >= n_tiles - 1 ? 2 * n_tiles - 1 : 2 * t + 2; };
 
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&tmap_q);
         prefetch_tmap(&tmap_kv);
         mbar_init(q_full, 1);
-        for (int i = 0; i < kSpStages; ++i) {
-            mbar_init(&kv_full[i], 1);
-            mbar_init(&kv_empty[i], 1);
+        for (int i = 0; i < slots; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
         }
-        mbar_init(s_full, 1);
-        mbar_init(p_full, 8);
-        mbar_init(o_full, 1);
-        mbar_init(s_empty, 8);
+        for (int h = 0; h < 2; ++h) {
+            mbar_init(&s_full[h], 1);
+            mbar_init(&p_full[h], 4);
+            mbar_init(&o_full[h], 1);
+        }
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc<TMEM_COLS>(tmem_slot);
+        tmem_alloc<512>(tmem_slot);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const uint32_t tmem_s = tmem_base;
-    const uint32_t tmem_o = tmem_base + 128;
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (lane == 0 && n_tiles > 0) {
             // tile row = token * G + head in group; rows behind the last whole token of 128 are never written, nor stored
-            mbar_expect_tx(q_full, PANELS * a.tile_tokens * G * 128);
+            mbar_expect_tx(q_full, (two ? 2 : 1) * PANELS * a.tile_tokens * G * 128);
+            for (int q = 0; q < (two ? 2 : 1); ++q)
 #pragma unroll
-            for (int p = 0; p < PANELS; ++p)
-                tma_load_3d(q_sm + p * PANEL_BYTES, &tmap_q, q_full, p * 64, kvh * G, tile.y, kEvictFirst);
+                for (int p = 0; p < PANELS; ++p)
+                    tma_load_3d(q_sm + q * TILE_BYTES + p * PANEL_BYTES, &tmap_q, q_full, p * 64, kvh * G, tile.y + q * a.tile_tokens, kEvictFirst);
             const int32_t* table = a.block_tables + static_cast<int64_t>(tile.x) * a.max_blocks_per_seq;
             const int n_blocks = prefix / bs;
-            uint32_t stage = 0, phase = 0;
-            for (int ti = 0; ti < n_tiles; ++ti) {
-                mbar_wait(&kv_empty[stage], phase ^ 1);
-                uint8_t* kdst = kv_sm + stage * 2 * TILE_BYTES;
-                uint8_t* vdst = kdst + TILE_BYTES;
-                mbar_expect_tx(&kv_full[stage], 2 * TILE_BYTES);
+            uint32_t slot = 0, phase = 0;
+            auto load = [&](int t, int which) {
+                mbar_wait(&empty[slot], phase ^ 1);
+                uint8_t* dst = ring + slot * TILE_BYTES;
+                mbar_expect_tx(&full[slot], TILE_BYTES);
                 for (int b = 0; b < bps; ++b) {
-                    const int bi = (t0 + ti) * bps + b;
-                    int krow = a.num_rows_kv, vrow = a.num_rows_kv;      // behind the cache: zeros
-                    if (bi < n_blocks) {
-                        const int blk = table[bi];
-                        krow = ((blk * 2 + 0) * a.n_kv_heads + kvh) * bs;
-                        vrow = ((blk * 2 + 1) * a.n_kv_heads + kvh) * bs;
-                    }
+                    const int bi = (t0 + t) * bps + b;
+                    const int row = bi < n_blocks ? ((table[bi] * 2 + which) * a.n_kv_heads + kvh) * bs : a.num_rows_kv;      // behind the cache: zeros
 #pragma unroll
-                    for (int p = 0; p < PANELS; ++p) {
-                        tma_load_2d(kdst + p * PANEL_BYTES + b * bs * 128, &tmap_kv, &kv_full[stage], p * 64, krow, kEvictNormal);
-                        tma_load_2d(vdst + p * PANEL_BYTES + b * bs * 128, &tmap_kv, &kv_full[stage], p * 64, vrow, kEvictNormal);
-                    }
+                    for (int p = 0; p < PANELS; ++p) tma_load_2d(dst + p * PANEL_BYTES + b * bs * 128, &tmap_kv, &full[slot], p * 64, row, kEvictNormal);
                 }
-                if (++stage == kSpStages) {
-                    stage = 0;
+                if (++slot == static_cast<uint32_t>(slots)) {
+                    slot = 0;
                     phase ^= 1;
                 }
+            };
+            load(0, 0);
+            if (n_tiles > 1) load(1, 0);
+            for (int t = 0; t < n_tiles; ++t) {
+                load(t, 1);
+                if (t + 2 < n_tiles) load(t + 2, 0);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            auto issue_qk = [&](uint32_t stage) {
-                const uint8_t* ktile = kv_sm + stage * 2 * TILE_BYTES;
+        if (lane == 0 && n_tiles > 0) {
+            auto wait_full = [&](int seq) { mbar_wait(&full[seq % slots], (seq / slots) & 1); };
+            auto issue_qk = [&](int h, int seq) {
+                const uint8_t* ktile = ring + (seq % slots) * TILE_BYTES;
+                const uint8_t* qtile = q_sm + (two ? h : 0) * TILE_BYTES;
 #pragma unroll
                 for (int p = 0; p < PANELS; ++p) {
-                    const uint64_t dq = make_desc_kmajor_sw128(smem_u32(q_sm + p * PANEL_BYTES));
+                    const uint64_t dq = make_desc_kmajor_sw128(smem_u32(qtile + p * PANEL_BYTES));
                     const uint64_t dk = make_desc_kmajor_sw128(smem_u32(ktile + p * PANEL_BYTES));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        umma_f16_ss(tmem_s, dq + 2 * k, dk + 2 * k, IDESC_QK, (p > 0 || k > 0) ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k) umma_f16_ss(tmem_base + h * 128, dq + 2 * k, dk + 2 * k, IDESC_QK, (p > 0 || k > 0) ? 1u : 0u);
                 }
-                umma_commit(s_full);
+                umma_commit(&s_full[h]);
+            };
+            auto issue_pv = [&](int h, int seq, bool first) {
+                const uint8_t* vtile = ring + (seq % slots) * TILE_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < kSpTok / 16; ++kk)
+                    umma_f16_ts(tmem_base + 256 + h * 128, tmem_base + h * 128 + kk * 8,
+                                make_desc_mnmajor_sw128(smem_u32(vtile + kk * 16 * 128), PANEL_BYTES), IDESC_PV, (!first || kk > 0) ? 1u : 0u);
             };
             mbar_wait(q_full, 0);
-            mbar_wait(&kv_full[0], 0);
+            wait_full(0);
             tc_fence_after();
-            issue_qk(0);
-            uint32_t stage = 0, phase = 0;
-            for (int ti = 0; ti < n_tiles; ++ti) {
-                const uint32_t nstage = (stage + 1 == kSpStages) ? 0 : stage + 1;
-                const uint32_t nphase = (stage + 1 == kSpStages) ? phase ^ 1 : phase;
-                if (ti + 1 < n_tiles) {      // S of the next tile as soon as the softmax warps hold this one's
-                    mbar_wait(s_empty, ti & 1);
-                    mbar_wait(&kv_full[nstage], nphase);
-                    tc_fence_after();
-                    issue_qk(nstage);
-                }
-                mbar_wait(p_full, ti & 1);
-                tc_fence_after();
-                const uint8_t* vtile = kv_sm + stage * 2 * TILE_BYTES + TILE_BYTES;
+            issue_qk(0, 0);
+            if (two) {
+                issue_qk(1, 0);
+                umma_commit(&empty[0]);
+                for (int t = 0; t < n_tiles; ++t) {
+                    const bool more = t + 1 < n_tiles;
+                    const int sv = seq_v(t), sk = seq_k(t + 1);
+                    if (more) wait_full(sk);
+                    wait_full(sv);
 #pragma unroll
-                for (int kk = 0; kk < kSpTok / 16; ++kk) {
-                    const uint64_t dp = make_desc_kmajor_sw128(smem_u32(p_sm + (kk >> 2) * PANEL_BYTES)) + 2 * (kk & 3);
-                    const uint64_t dv = make_desc_mnmajor_sw128(smem_u32(vtile + kk * 16 * 128), PANEL_BYTES);
-                    umma_f16_ss(tmem_o, dp, dv, IDESC_PV, (ti > 0 || kk > 0) ? 1u : 0u);
+                    for (int h = 0; h < 2; ++h) {
+                        mbar_wait(&p_full[h], t & 1);
+                        tc_fence_after();
+                        issue_pv(h, sv, t == 0);
+                        if (h == 1) umma_commit(&empty[sv % slots]);
+                        if (more) issue_qk(h, sk);
+                        else umma_commit(&o_full[h]);
+                    }
+                    if (more) umma_commit(&empty[sk % slots]);
                 }
-                umma_commit(o_full);
-                umma_commit(&kv_empty[stage]);
-                stage = nstage;
-                phase = nphase;
+            } else {
+                umma_commit(&empty[0]);
+                if (n_tiles > 1) {
+                    wait_full(1);
+                    tc_fence_after();
+                    issue_qk(1, 1);
+                    umma_commit(&empty[1 % slots]);
+                }
+                for (int t = 0; t < n_tiles; ++t) {
+                    const int h = t & 1, sv = seq_v(t);
+                    wait_full(sv);
+                    mbar_wait(&p_full[h], (t >> 1) & 1);
+                    tc_fence_after();
+                    issue_pv(h, sv, t < 2);
+                    umma_commit(&empty[sv % slots]);
+                    if (t + 2 < n_tiles) {
+                        const int sk = seq_k(t + 2);
+                        wait_full(sk);
+                        tc_fence_after();
+                        issue_qk(h, sk);
+                        umma_commit(&empty[sk % slots]);
+                    } else {
+                        umma_commit(&o_full[h]);
+                    }
+                }
             }
         }
     } else {
-        const uint32_t quad = warp & 3;              // TMEM lane quadrant
-        const uint32_t half = (warp - 2) >> 2;       // which 64 key columns, and which half of the output dims
+        // ===================== softmax / partial output: one thread per row =====================
+        const uint32_t quad = warp & 3;              // TMEM lane quadrant this warp may touch
+        const int h = (warp - 2) >> 2;               // stream
         const int r = quad * 32 + lane;
-        const bool quad_live = static_cast<int>(quad * 32) < n_live_rows;   // warp-uniform, same for both halves
-        const uint32_t lane_addr = (quad * 32u) << 16;
-        constexpr int HC = kSpTok / 2;
-        constexpr int HD2 = D / 2;
-        float m_run = -INFINITY, l_run = 0.0f;       // m_run in log2 units, of scores as they are summed up (kUpLog2 not in it)
-        uint8_t* p_row = p_sm + half * PANEL_BYTES + r * 128;
+        const int row0 = tile.y + (two ? h * a.tile_tokens : 0);
+        const int live_rows = (two ? (h == 0 ? a.tile_tokens : tile.z - a.tile_tokens) : tile.z) * G;
+        const bool quad_live = static_cast<int>(quad * 32) < live_rows;   // warp-uniform
+        const int steps = two ? n_tiles : (n_tiles - h + 1) >> 1;
+        const uint32_t tmem_s = tmem_base + h * 128 + ((quad * 32u) << 16);
+        const uint32_t tmem_o = tmem_s + 256;
         constexpr float kRescaleThreshold = 8.0f;
-        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
-        for (int ti = 0; ti < n_tiles; ++ti) {
-            const int left = prefix - (t0 + ti) * kSpTok - static_cast<int>(half) * HC;      // keys from my first column on
-            mbar_wait(s_full, ti & 1);
+        float m_run = -INFINITY, l_run = 0.0f;       // m_run in log2 units, kUpLog2 not in it
+        for (int i = 0; i < steps; ++i) {
+            mbar_wait(&s_full[h], i & 1);
             tc_fence_after();
-            if (!quad_live) {     // keeps the barriers going
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s_empty);
-                if (ti > 0) {
-                    mbar_wait(o_full, (ti - 1) & 1);
-                    tc_fence_after();
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full);
+            if (!quad_live) {
+                if (lane == 0) mbar_arrive(&p_full[h]);
                 continue;
             }
-            uint32_t sr[HC];
+            const int left = prefix - (t0 + (two ? i : 2 * i + h)) * kSpTok;      // keys from the tile's first on
+            uint32_t sr[128];
 #pragma unroll
-            for (int c = 0; c < HC; c += 32)
-                tmem_ld_32x32(tmem_s + lane_addr + half * HC + c, *reinterpret_cast<uint32_t(*)[32]>(&sr[c]));
+            for (int c = 0; c < 128; c += 32) tmem_ld_32x32(tmem_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sr[c]));
             tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(s_empty);
-            float tmax = -INFINITY;
-            if (left < HC) {
+            if (left < kSpTok) {
 #pragma unroll
-                for (int j = 0; j < HC; ++j)
+                for (int j = 0; j < 128; ++j)
                     if (j >= left) sr[j] = __float_as_uint(-INFINITY);
             }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < HC; ++j) tmax = fmaxf(tmax, __uint_as_float(sr[j]));
-            float* x = xch + (ti & 1) * 256;
-            x[half * 128 + r] = tmax;
-            pair_sync();
-            tmax = fmaxf(tmax, x[(half ^ 1) * 128 + r]);
+            for (int j = 0; j < 128; j += 8)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sr[j + 2 * q]), __uint_as_float(sr[j + 2 * q + 1])));
+            const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
             const float m_cand = fmaxf(m_run, tmax * a.scale_log2);
-            const bool grow = (m_cand > m_run + kRescaleThreshold) || (m_run == -INFINITY && m_cand != -INFINITY);
-            const float m_new = grow ? m_cand : m_run;
             const bool fresh = (m_run == -INFINITY);
+            const bool grow = (m_cand > m_run + kRescaleThreshold) || (fresh && m_cand != -INFINITY);
+            const float m_new = grow ? m_cand : m_run;
             const float alpha = (!grow || fresh) ? (grow ? 0.0f : 1.0f) : sp_ex2(m_run - m_new);
             const float m_sub = ((m_new == -INFINITY) ? 0.0f : m_new) - kUpLog2;
-            uint32_t packed[HC / 2];
-            float ps0 = 0.0f, ps1 = 0.0f;
-#pragma unroll
-            for (int j = 0; j < HC; j += 2) {
-                const float p0 = sp_ex2(fmaf(__uint_as_float(sr[j]), a.scale_log2, -m_sub));
-                const float p1 = sp_ex2(fmaf(__uint_as_float(sr[j + 1]), a.scale_log2, -m_sub));
-                ps0 += p0;
-                ps1 += p1;
-                packed[j >> 1] = pack2<kBf16>(p0, p1);
-            }
-            l_run = l_run * alpha + (ps0 + ps1);
             m_run = m_new;
-            const bool rescale = grow && !fresh;
-            if (ti > 0) {     // P V of the previous tile is complete before P is overwritten or O rescaled
-                mbar_wait(o_full, (ti - 1) & 1);
-                tc_fence_after();
-                if (__any_sync(0xffffffffu, rescale)) {
-                    const float f = rescale ? alpha : 1.0f;
+            if (i > 0 && __any_sync(0xffffffffu, grow && !fresh)) {     // (S has arrived: P V of the tile before is done)
+                const float f = grow && !fresh ? alpha : 1.0f;
 #pragma unroll
-                    for (int c = 0; c < HD2; c += 32) {
-                        uint32_t orr[32];
-                        tmem_ld_32x32(tmem_o + lane_addr + half * HD2 + c, orr);
-                        tmem_ld_wait();
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t orr[16];
+                    tmem_ld_32x16(tmem_o + c, orr);
+                    tmem_ld_wait();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) orr[j] = __float_as_uint(__uint_as_float(orr[j]) * f);
-                        tmem_st_32x32(tmem_o + lane_addr + half * HD2 + c, orr);
-                    }
-                    tmem_st_wait();
+                    for (int j = 0; j < 16; ++j) orr[j] = __float_as_uint(__uint_as_float(orr[j]) * f);
+                    tmem_st_32x16(tmem_o + c, orr);
                 }
             }
+            const uint64_t k2 = sp_pack(a.scale_log2, a.scale_log2), m2 = sp_pack(-m_sub, -m_sub);
+            uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-            for (int ch = 0; ch < HC / 8; ++ch) {
-                const uint4 v = make_uint4(packed[4 * ch], packed[4 * ch + 1], packed[4 * ch + 2], packed[4 * ch + 3]);
-                *reinterpret_cast<uint4*>(p_row + ((ch ^ (r & 7)) << 4)) = v;
+            for (int c = 0; c < 128; c += 64) {
+                uint32_t packed[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float x0, x1;
+                    sp_unpack(sp_fma(sp_pack(__uint_as_float(sr[c + 2 * j]), __uint_as_float(sr[c + 2 * j + 1])), k2, m2), x0, x1);
+                    x0 = sp_ex2(x0);
+                    x1 = sp_ex2(x1);
+                    sum[j & 1] = sp_add(sum[j & 1], sp_pack(x0, x1));
+                    packed[j] = pack2<kBf16>(x0, x1);
+                }
+                tmem_st_32x32(tmem_s + c / 2, packed);
             }
+            float u0, u1;
+            sp_unpack(sp_add(sum[0], sum[1]), u0, u1);
+            l_run = l_run * alpha + (u0 + u1);
+            tmem_st_wait();
             tc_fence_before();
-            fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(&p_full[h]);
         }
-        if (quad_live) {
-            float* x = xch + (n_tiles & 1) * 256;
-            x[half * 128 + r] = l_run;
-            pair_sync();
-            l_run += x[(half ^ 1) * 128 + r];
-        }
-        mbar_wait(o_full, (n_tiles - 1) & 1);
-        tc_fence_after();
+        // ---- parts: number `split` and, of the second key stream, p_splits + split (nothing in it with two row tiles) ----
         const int tok = r / G;
-        const int64_t at = (static_cast<int64_t>(split) * a.rows + tile.y + tok) * a.n_q_heads + kvh * G + (r - tok * G);
+        const int64_t place = static_cast<int64_t>(row0 + tok) * a.n_q_heads + kvh * G + (r - tok * G);
+        const int64_t part = static_cast<int64_t>(a.rows) * a.n_q_heads;
+        const int64_t at = (two ? split : h * a.p_splits + split) * part + place;
+        if (r < live_rows) {
+            *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m_run - kUpLog2, l_run);
+            if (two) *reinterpret_cast<float2*>(a.ws_ml + ((a.p_splits + split) * part + place) * 2) = make_float2(-INFINITY, 0.0f);
+        }
+        if (steps > 0) {
+            mbar_wait(&o_full[h], 0);
+            tc_fence_after();
+            if (quad_live) {
 #pragma unroll
-        for (int c = 0; c < HD2; c += 32) {
-            uint32_t orr[32];
-            tmem_ld_32x32(tmem_o + lane_addr + half * HD2 + c, orr);
-            tmem_ld_wait();
-            if (r < n_live_rows) {
-                float4* wo = reinterpret_cast<float4*>(a.ws_o + at * D + half * HD2 + c);
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t orr[32];
+                    tmem_ld_32x32(tmem_o + c, orr);
+                    tmem_ld_wait();
+                    if (r < live_rows) {
+                        float4* wo = reinterpret_cast<float4*>(a.ws_o + at * D + c);
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    wo[j >> 2] = make_float4(__uint_as_float(orr[j]), __uint_as_float(orr[j + 1]), __uint_as_float(orr[j + 2]), __uint_as_float(orr[j + 3]));
+                        for (int j = 0; j < 32; j += 4)
+                            wo[j >> 2] = make_float4(__uint_as_float(orr[j]), __uint_as_float(orr[j + 1]), __uint_as_float(orr[j + 2]), __uint_as_float(orr[j + 3]));
+                    }
+                }
             }
         }
-        tc_fence_before();
-        if (r < n_live_rows && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m_run - kUpLog2, l_run);
     }
 
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc<TMEM_COLS>(tmem_base);
+        tmem_dealloc<512>(tmem_base);
     }
 }
 
@@ -367,8 +396,9 @@ __device__ __forceinline__ float2 own_load2(const void* p, uint32_t cta) {
 struct OwnJoin {
     float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     __device__ __forceinline__ void add(float pm, float pl, const float4& x) {
+        if (pm == -INFINITY) return;       // (x may be anything)
         const float mx = fmaxf(m, pm);
-        const float w0 = m == -INFINITY ? 0.0f : sp_ex2(m - mx), w1 = pm == -INFINITY ? 0.0f : sp_ex2(pm - mx);
+        const float w0 = m == -INFINITY ? 0.0f : sp_ex2(m - mx), w1 = sp_ex2(pm - mx);
         l = l * w0 + pl * w1;
         o[0] = o[0] * w0 + x.x * w1;
         o[1] = o[1] * w0 + x.y * w1;
@@ -397,7 +427,8 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tmap_kv, const SharedArgs 
     __shared__ __align__(16) float cta_o[kOwnRows][D];
     __shared__ __align__(8) float cta_ml[kOwnRows][2];
 
-    pdl_enter();
+    // with a prefix the kernel before is ours, and what came before that one is done: only its parts are waited for, below
+    if (!a.has_prefix) pdl_enter();
     const int tid = threadIdx.x;
     const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int splits = gridDim.x, split = blockIdx.x;
@@ -407,7 +438,10 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tmap_kv, const SharedArgs 
     const int G = a.n_q_heads / a.n_kv_heads;
     const int first_row = (blockIdx.z - kvh * a.row_tiles) * kOwnRows;          // of the item's (token, head) rows
     const int rows = min(item.z * G - first_row, kOwnRows);
-    if (rows <= 0) return;        // (for the whole cluster)
+    if (rows <= 0) {              // (for the whole cluster)
+        if (a.has_prefix) pdl_enter();      // (who waits for this kernel waits for the one before)
+        return;
+    }
     const int kv_len = item.w;
     const int strips = (kv_len - prefix + kOwnStrip - 1) / kOwnStrip;
     const int per = (strips + splits - 1) / splits;
@@ -568,15 +602,22 @@ shared_own_kernel(const __grid_constant__ CUtensorMap tmap_kv, const SharedArgs 
             }
     }
     __syncthreads();
-    const int eff = prefix > 0 ? ((prefix + kSpTok - 1) / kSpTok + sp_tiles_per_split(prefix, a.p_splits) - 1) / sp_tiles_per_split(prefix, a.p_splits) : 0;
+    if (a.has_prefix) pdl_enter();
     // the prefix' parts join, and the row is finished
     auto finish = [&](int r, int dd, OwnJoin& j) {
         const int tok = (first_row + r) / G, head = kvh * G + (first_row + r) % G;
         const int64_t row = item.y + tok;
-        for (int sp = 0; sp < eff; ++sp) {
-            const int64_t at = (static_cast<int64_t>(sp) * a.rows + row) * a.n_q_heads + head;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.ws_ml + at * 2));
-            j.add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(a.ws_o + at * D + dd)));
+        const int64_t part = static_cast<int64_t>(a.rows) * a.n_q_heads, place = row * a.n_q_heads + head;
+        for (int sp = 0; prefix > 0 && sp < 2 * a.p_splits; sp += 8) {        // eight parts' loads at once
+            float2 ml[8];
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ml[i] = sp + i < 2 * a.p_splits ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml + ((sp + i) * part + place) * 2)) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (ml[i].x != -INFINITY) x[i] = __ldcg(reinterpret_cast<const float4*>(a.ws_o + ((sp + i) * part + place) * D + dd));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) j.add(ml[i].x, ml[i].y, x[i]);
         }
         uint2 v;
         v.x = pack2<kBf16>(j.o[0] / j.l, j.o[1] / j.l);
@@ -618,11 +659,11 @@ static int launch_shared(const CUtensorMap& tq, const CUtensorMap& tkv, const CU
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        HDS_CHECK_CUDA(cudaFuncSetAttribute(pre, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sp_smem_bytes<D>())));
+        HDS_CHECK_CUDA(cudaFuncSetAttribute(pre, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sp_smem_bytes(D))));
         HDS_CHECK_CUDA(cudaFuncSetAttribute(own, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem_bytes(D)));
         configured[dev & 63] = true;
     }
-    if (n_tiles > 0) HDS_CHECK_CUDA(launch_kernel(pre, dim3(n_tiles, a.n_kv_heads, a.p_splits), dim3(kSpThreads), sp_smem_bytes<D>(), s, tq, tkv, a));
+    if (n_tiles > 0) HDS_CHECK_CUDA(launch_kernel(pre, dim3(n_tiles, a.n_kv_heads, a.p_splits), dim3(kSpThreads), sp_smem_bytes(D), s, tq, tkv, a));
     HDS_CHECK_CUDA(launch_kernel_cluster(own, o_splits, dim3(o_splits, n_items, a.n_kv_heads * a.row_tiles), dim3(kOwnWarps * 32), own_smem_bytes(D),
                                          s, tstrip, a));
     return HDS_OK;
@@ -633,7 +674,7 @@ static int launch_shared(const CUtensorMap& tq, const CUtensorMap& tkv, const CU
 using namespace hds;
 
 extern "C" int64_t hds_paged_attention_shared_workspace_bytes(int rows, int n_q_heads, int head_dim, int p_splits) {
-    return static_cast<int64_t>(rows) * n_q_heads * (head_dim + 2) * 4 * p_splits;
+    return static_cast<int64_t>(rows) * n_q_heads * (head_dim + 2) * 4 * 2 * p_splits;
 }
 
 extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out, int64_t ld_out, int rows, const void* kv_cache_layer,
@@ -673,9 +714,10 @@ extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out
     a.num_rows_kv = static_cast<int>(kv_rows);
     a.tile_tokens = 128 / G;
     a.p_splits = p_splits;
+    a.has_prefix = n_tiles > 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.ws_o = reinterpret_cast<float*>(workspace);       // the outputs first: they want 16-byte boundaries
-    a.ws_ml = a.ws_o + static_cast<int64_t>(p_splits) * rows * n_q_heads * head_dim;
+    a.ws_ml = a.ws_o + static_cast<int64_t>(2 * p_splits) * rows * n_q_heads * head_dim;
     CUtensorMap tq, tkv, tstrip;
     memset(&tq, 0, sizeof(tq));
     int rc;

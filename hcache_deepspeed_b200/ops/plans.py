@@ -79,7 +79,7 @@ class SharedPrefixPlan:
         prefix = np.zeros(new.size, dtype=np.int64)
         row0 = np.concatenate([[0], np.cumsum(new)])
         taken = np.zeros(new.size, dtype=bool)
-        tile_tokens, tiles = 128 // (n_q_heads // n_kv_heads), []
+        tile_tokens, tiles = 2 * (128 // (n_q_heads // n_kv_heads)), []
         for first, n, length in self.groups:
             if first < 0 or n < 1 or first + n > self.n_seqs or taken[first:first + n].any():
                 raise ValueError(f"group ({first}, {n}, {length}): sequences that are there, and in no other group")
@@ -112,11 +112,11 @@ class SharedPrefixPlan:
 
 
 def pick_prefix_splits(units: int, prefix: int, sms: int = 148) -> int:
-    """Parts of a prefix of that many tokens, ``units`` CTAs wide: the fewest waves of SMs, a CTA's beginning and end counted as a tile and a half."""
+    """Parts of a prefix of that many tokens, ``units`` CTAs wide: the fewest waves of SMs, a CTA's beginning and end counted as two tiles."""
     tiles = -(-prefix // 128)
     if units == 0 or tiles == 0:
         return 1
-    return min(range(1, min(64, tiles) + 1), key=lambda s: (-(-units * s // sms) * (-(-tiles // s) + 1.5), s))
+    return min(range(1, min(64, tiles) + 1), key=lambda s: (-(-units * s // sms) * (-(-tiles // s) + 2), s))
 
 
 def pick_own_splits(units: int, keys: int, sms: int = 148) -> int:

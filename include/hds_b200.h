@@ -545,7 +545,7 @@ int hds_adapter_parts(int n_tiles, int width);
 
 /* Paged attention of a batch whose sequences share prefixes. q and out: rows of n_q_heads * head_dim values, ld_q / ld_out apart; a group of
  * neighbouring sequences reads its prefix once. tiles int32 [n_tiles][4] = (sequence whose table names the prefix' pages, first row, tokens <=
- * 128 / (n_q_heads / n_kv_heads), prefix); items int32 [n_items][8] = (sequence, first row, new tokens, keys, prefix, 0, 0, 0): row t of them sees
+ * 2 * (128 / (n_q_heads / n_kv_heads)), prefix); items int32 [n_items][8] = (sequence, first row, new tokens, keys, prefix, 0, 0, 0): row t of them sees
  * the keys up to keys - new tokens + t. Prefixes are whole pages ahead of the new tokens. p_splits (up to 64): parts of a prefix, o_splits
  * (1 / 2 / 4 / 8): CTAs for a sequence's other keys. workspace: see below; nothing in it outlives the call. dtype 0 / 1. */
 int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out, int64_t ld_out, int rows, const void* kv_cache_layer, int64_t num_blocks,

@@ -76,7 +76,7 @@ def test_prefix_plan_lists_rows_and_lengths():
     assert plan.items[:, :5].tolist() == [[0, 0, 1, 40, 32], [1, 1, 0, 32, 32], [2, 1, 3, 70, 32], [3, 4, 2, 5, 0]]
     assert plan.n_tiles == 1      # four rows of 8 / 2 heads share a tile of 128
     wide = plans.SharedPrefixPlan([40] * 3, [200] * 3, [(0, 3, 128)], 8, 2, 64, 16)
-    assert wide.n_tiles == 4      # 120 tokens in tiles of 32
+    assert wide.n_tiles == 2      # 120 tokens in two tiles of 32 each
 
 
 @pytest.mark.parametrize("new,keys,groups,match", [
