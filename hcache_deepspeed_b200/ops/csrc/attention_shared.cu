@@ -12,10 +12,24 @@
 //      warps 2-9 : softmax, four warps per stream, one thread per row; P goes back to TMEM as 16-bit pairs, over the scores it came from. O stays in
 //                  TMEM and is rescaled only when a row's maximum grows by more than 2^8
 //    No causal edge: every row comes behind the whole prefix. (m, l, O) in fp32 go to scratch, one part per split and key stream.
-// 2. Own keys, and the end. A CTA has up to 8 query rows of a sequence and KV head; its warps take strips of 16 keys through rings of their
-//    own (TMA, three strips ahead, see attention_group.cu, whose arithmetic this is: mma.sync, the weights' rounding kept in the
-//    MMA's other 8 rows). Splits of a long sequence are a cluster and meet in its shared memory; there the prefix' parts join, and the rows are
-//    written. The scratch has no counters and no state between calls.
+// 2. Own keys. The warps of a CTA are twelve workers: each takes strips of 16 keys through a ring of its own (TMA, see attention_group.cu, whose
+//    arithmetic this is: up to 8 query rows of a sequence and KV head, mma.sync, the weights' rounding kept in the MMA's other 8 rows). All
+//    strips of all sequences and heads stand in one line that is cut into pieces of equal cost, one per worker, so that neither long nor short sequences
+//    leave SMs idle; a sequence and head costs two strips more than it has, for its beginning and end (with pieces of equal length the worker of the many
+//    heads of a short sequence came 25 us behind the others). (m, l, O) of a sequence's share in a piece goes to scratch.
+//    These CTAs are of the prefix' launch and begin with it, on so many SMs that both should end together: own keys wait for memory where
+//    the prefix waits for its softmax. (One after the other, 4096 shared keys and 32 sequences of 32 heads with 150 keys each took 41.4 us, 64 sequences
+//    of 64 heads behind 8192 keys 48.0; together 35.7 and 42.3.)
+// 3. The end: the parts of every row, from prefix and own keys, join in a kernel of their own. The scratch has no counters and no state between calls.
+//
+// Measured (bf16, bytes that any form has to move, time, bytes per second; a copy runs at 6.55 TB/s):
+//   32 sequences, 32 heads of 128 dims and as many KV heads, prefix 4096, 1 to 300 own keys: 147 MB, 35.7 us, 4.1 TB/s
+//   64 sequences, 64 heads on 8, prefix 8192, 1 to 600 own keys:                             118 MB, 42.3 us, 2.8 TB/s: the prefix' softmax, see below
+//   77 sequences, 32 heads on 8, up to 3 new tokens, prefixes 2048 and 1024, 1 to 500 own:    93 MB, 34.8 us, 2.7 TB/s: own keys once per 8 rows, 2 and 3 tokens have 12
+//   9 sequences, 64 heads on 8, prefix 65536, 1 to 1500 own keys:                             294 MB, 61.6 us, 4.8 TB/s
+//   4 sequences, 12 heads of 64 dims (fp16), prefix 512, 1 to 90 own keys:                    9.5 us: two kernels' beginnings, 5 us + 3 us
+// A key tile takes a CTA 1.3 us, or 2.9 us under two row tiles, where products and exponentials alone are 0.55 and 1.07 us: the way of one stream's
+// scores from TMEM through maximum, weights and back is 2.5 us long, and TMEM has room for two streams.
 //
 // P is rounded to 16 bits in the first part: each weight by half a step of its own (2^-9 in bf16, 2^-12 in fp16, where the weights are held 2^7
 // larger so that small ones keep their bits), which averages out over the keys; sums are of the unrounded weights.
@@ -29,11 +43,11 @@
 
 namespace hds {
 
-constexpr int kSpThreads = 320;   // TMA warp + MMA warp + 2 x 4 softmax warps
+constexpr int kSpThreads = 384;   // TMA warp + MMA warp + 2 x 4 softmax warps; or 12 workers
 constexpr int kSpTok = 128;       // keys of a tile, rows of a stream
-constexpr int kOwnRows = 8;       // query rows of a CTA of the second part
+constexpr int kOwnRows = 8;       // query rows of a worker
 constexpr int kOwnStrip = 16;     // keys a warp takes at a time; pages hold a multiple
-constexpr int kOwnWarps = 4;
+constexpr int kOwnWarps = 12;     // workers of a CTA
 
 struct SharedArgs {
     const void* q;
@@ -42,14 +56,19 @@ struct SharedArgs {
     const int32_t* block_tables;
     int max_blocks_per_seq;
     const int4* tiles;      // prefix: (sequence whose table names the pages, first query row, tokens of up to two streams, prefix length)
-    const int4* items;      // own keys: pairs (sequence, first query row, tokens, keys), (prefix length, 0, 0, 0)
+    const int4* items;      // own keys: pairs (sequence, first query row, tokens, keys), (prefix length, first unit, row tiles, 0)
+    const int4* workers;    // (item, unit in the item, first strip in the unit, strips)
+    const int2* units;      // (first worker, last worker) of a unit: (item, KV head, row tile)
+    const int32_t* row_items;   // the item of a query row
+    int n_tiles, n_workers, prefix_ctas;
     int rows, n_q_heads, n_kv_heads, block_size, bs_log2, num_rows_kv;
     int tile_tokens;        // tokens of a stream of rows
-    int p_splits, row_tiles;
-    int has_prefix;         // the first kernel runs
+    int p_splits;
     float scale_log2;
     float* ws_ml;           // [2 p_splits][rows][n_q_heads][2]; m = -inf: nothing in ws_o
     float* ws_o;            // [2 p_splits][rows][n_q_heads][D]
+    float* own_ml;          // [units + workers][8][2]: a worker's share of a unit has number unit + worker
+    float* own_o;           // [units + workers][8][D]
 };
 
 __device__ __forceinline__ float sp_ex2(float x) {
@@ -79,8 +98,7 @@ __device__ __forceinline__ uint64_t sp_add(uint64_t a, uint64_t b) {
 }
 
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(kSpThreads, 1)
-shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const SharedArgs a) {
+__device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const CUtensorMap& tmap_kv, const SharedArgs& a, uint8_t* smem, int block) {
     constexpr int PANELS = D / 64;
     constexpr int PANEL_BYTES = kSpTok * 128;
     constexpr int TILE_BYTES = PANELS * PANEL_BYTES;
@@ -89,8 +107,6 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     constexpr uint32_t IDESC_PV = make_idesc_f16(128, D, kBf16, false, true);
     constexpr float kUpLog2 = kBf16 ? 0.0f : 7.0f;     // (2^8 of a stale maximum and these stay below fp16's 2^16)
 
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sp_tiles(D) * TILE_BYTES);
     uint64_t* q_full = bars;
     uint64_t* full = bars + 1;
@@ -102,11 +118,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     static_assert((1 + 2 * MAX_SLOTS + 6) * 8 + 4 <= 512, "barriers have room");
 
     const uint32_t warp = warp_id(), lane = lane_id();
-    const int4 tile = a.tiles[blockIdx.x];      // (the plan: no kernel writes it)
-    // (in this order: the second kernel, which may start from here on, reads what came before this one without a wait)
-    griddep_wait();
-    griddep_launch_dependents();
-    const int kvh = blockIdx.y, split = blockIdx.z;
+    const int4 tile = a.tiles[block % a.n_tiles];
+    const int kvh = block / a.n_tiles % a.n_kv_heads, split = block / a.n_tiles / a.n_kv_heads;
     const int G = a.n_q_heads / a.n_kv_heads;
     const bool two = tile.z > a.tile_tokens;    // two row tiles; else one, whose key tiles the streams share
     const int prefix = tile.w;
@@ -250,7 +263,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                 }
             }
         }
-    } else {
+    } else if (warp < 10) {
         // ===================== softmax / partial output: one thread per row =====================
         const uint32_t quad = warp & 3;              // TMEM lane quadrant this warp may touch
         const int h = (warp - 2) >> 2;               // stream
@@ -348,10 +361,13 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
                     tmem_ld_32x32(tmem_o + c, orr);
                     tmem_ld_wait();
                     if (r < live_rows) {
-                        float4* wo = reinterpret_cast<float4*>(a.ws_o + at * D + c);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            wo[j >> 2] = make_float4(__uint_as_float(orr[j]), __uint_as_float(orr[j + 1]), __uint_as_float(orr[j + 2]), __uint_as_float(orr[j + 3]));
+                        for (int j = 0; j < 32; j += 8) {       // 32 bytes at a time: whole sectors
+                            float v[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(orr[j + e]);
+                            st_v8_f32(a.ws_o + at * D + c + j, v);
+                        }
                     }
                 }
             }
@@ -366,306 +382,334 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     }
 }
 
-// ---- own keys, and the end ---------------------------------------------------------------------------------------------
-__host__ __device__ constexpr int own_stages(int d) { return d == 128 ? 3 : 6; }
-__host__ __device__ constexpr int own_slot_bytes(int d) { return 2 * kOwnStrip * d * 2; }      // K and V of a strip
-__host__ __device__ constexpr int own_smem_bytes(int d) { return kOwnWarps * own_stages(d) * own_slot_bytes(d) + 1024; }
+// ---- own keys ----------------------------------------------------------------------------------------------------------
+__host__ __device__ constexpr int own_stages(int d) { return d == 128 ? 2 : 4; }
+__host__ __device__ constexpr int own_half_bytes(int d) { return kOwnStrip * d * 2; }      // K or V of a strip
+__host__ __device__ constexpr int own_ring_bytes(int d) { return 2 * own_stages(d) * own_half_bytes(d); }
+static_assert(kOwnWarps * (own_ring_bytes(128) + 128) <= sp_tiles(128) * kSpTok * 128 * 2 &&
+              kOwnWarps * (own_ring_bytes(64) + 128) <= sp_tiles(64) * kSpTok * 64 * 2, "the rings fit");
 
-__device__ __forceinline__ uint32_t own_cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void own_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ float4 own_load4(const void* p, uint32_t cta) {
-    float4 v;
-    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %4, %5;\n\tld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [ra];\n\t}\n"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(smem_u32(p)), "r"(cta) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 own_load2(const void* p, uint32_t cta) {
-    float2 v;
-    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [ra];\n\t}\n"
-                 : "=f"(v.x), "=f"(v.y) : "r"(smem_u32(p)), "r"(cta) : "memory");
-    return v;
-}
-
-// a running (m, l, four outputs) and one more part of the same row
-struct OwnJoin {
-    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    __device__ __forceinline__ void add(float pm, float pl, const float4& x) {
-        if (pm == -INFINITY) return;       // (x may be anything)
-        const float mx = fmaxf(m, pm);
-        const float w0 = m == -INFINITY ? 0.0f : sp_ex2(m - mx), w1 = sp_ex2(pm - mx);
-        l = l * w0 + pl * w1;
-        o[0] = o[0] * w0 + x.x * w1;
-        o[1] = o[1] * w0 + x.y * w1;
-        o[2] = o[2] * w0 + x.z * w1;
-        o[3] = o[3] * w0 + x.w * w1;
-        m = mx;
-    }
-};
-
-// grid (splits, items, KV heads * row tiles), splits of an item being a cluster. Lane = 4 * g + t: row g of the MMA is query row g; t picks two of
-// every eight keys (as the rows of C and A have it), g the key of K (as the columns of B have it) and, for V, eight output dims.
+// Lane = 4 * g + t: row g of the MMA is query row g; t picks two of every eight keys (as the rows of C and A have it), g the key of K (as the
+// columns of B have it) and, for V, eight output dims.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(kOwnWarps * 32, 2)
-shared_own_kernel(const __grid_constant__ CUtensorMap tmap_kv, const SharedArgs a) {
-    constexpr int W = kOwnWarps;
+__device__ __forceinline__ void shared_own(const CUtensorMap& tmap_kv, const SharedArgs& a, uint8_t* smem, int worker) {
     constexpr int KC = D / 32;        // 16-byte pieces of a K row per lane
     constexpr int VC = D / 64;        // 16-byte pieces of a V row per lane
-    constexpr int LD = D + 4;
     constexpr int ST = own_stages(D);
     constexpr float kUp = kBf16 ? 1.0f : 16384.0f;      // what a weight is multiplied by before it becomes 16 bits
-    static_assert(kOwnRows * LD * 4 <= ST * own_slot_bytes(D), "a warp's outputs fit its ring");
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t full[W][ST];
-    __shared__ float mg_ml[W][kOwnRows][2];
-    __shared__ __align__(16) float cta_o[kOwnRows][D];
-    __shared__ __align__(8) float cta_ml[kOwnRows][2];
-
-    // with a prefix the kernel before is ours, and what came before that one is done: only its parts are waited for, below
-    if (!a.has_prefix) pdl_enter();
-    const int tid = threadIdx.x;
-    const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int splits = gridDim.x, split = blockIdx.x;
-    const int4 item = a.items[2 * blockIdx.y];
-    const int prefix = a.items[2 * blockIdx.y + 1].x;
-    const int kvh = blockIdx.z / a.row_tiles;
-    const int G = a.n_q_heads / a.n_kv_heads;
-    const int first_row = (blockIdx.z - kvh * a.row_tiles) * kOwnRows;          // of the item's (token, head) rows
-    const int rows = min(item.z * G - first_row, kOwnRows);
-    if (rows <= 0) {              // (for the whole cluster)
-        if (a.has_prefix) pdl_enter();      // (who waits for this kernel waits for the one before)
-        return;
-    }
-    const int kv_len = item.w;
-    const int strips = (kv_len - prefix + kOwnStrip - 1) / kOwnStrip;
-    const int per = (strips + splits - 1) / splits;
-    const int s0 = split * per + warp, s1 = min(strips, split * per + per);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    if (warp >= kOwnWarps || worker >= a.n_workers) return;
+    uint8_t* ring = smem + warp * own_ring_bytes(D);        // [slot][K, V][panel][16 x 64]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOwnWarps * own_ring_bytes(D)) + warp * 2 * ST;        // [slot][K, V]
     if (lane == 0) {
-        if (warp == 0) prefetch_tmap(&tmap_kv);
-        for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
+        prefetch_tmap(&tmap_kv);
+        for (int i = 0; i < 2 * ST; ++i) mbar_init(&full[i], 1);
         fence_barrier_init();
     }
     __syncwarp();
-
-    // ---- my query row, pieces of 8 dims permuted as K's are ----
-    const bool live = g < rows;
-    const int r_tok = live ? (first_row + g) / G : 0, r_head = kvh * G + (live ? (first_row + g) % G : 0);
-    const int q_pos = kv_len - item.z + r_tok;
-    uint4 q[KC];
-    {
-        const char* qp = reinterpret_cast<const char*>(a.q) + ((static_cast<int64_t>(item.y) + r_tok) * a.ld_q + r_head * D) * 2 + t * 32;
+    const int G = a.n_q_heads / a.n_kv_heads;
+    int n = 0;                           // strips so far: strip n has slot n % ST
+    int4 job = a.workers[worker];        // (item, unit in the item, first strip in the unit, strips)
+    while (job.w > 0) {
+        const int4 item = a.items[2 * job.x], more = a.items[2 * job.x + 1];
+        const int prefix = more.x, row_tiles = more.z, kv_len = item.w;
+        const int kvh = job.y / row_tiles, first_row = (job.y - kvh * row_tiles) * kOwnRows;       // of the item's (token, head) rows
+        const int rows = min(item.z * G - first_row, kOwnRows);
+        const int strips = (kv_len - prefix + kOwnStrip - 1) / kOwnStrip;
+        const int s0 = job.z, s1 = min(strips, s0 + job.w);
+        const int32_t* table = a.block_tables + static_cast<int64_t>(item.x) * a.max_blocks_per_seq;
+        auto first_key = [&](int s) { return prefix + s * kOwnStrip; };
+        auto page_of = [&](int s) { return s < s1 ? table[first_key(s) >> a.bs_log2] : 0; };
+        auto load = [&](int s, int blk, int to, int which) {     // (one lane)
+            uint8_t* dst = ring + (2 * to + which) * own_half_bytes(D);
+            const int row = (((blk * 2 + which) * a.n_kv_heads + kvh) << a.bs_log2) + (first_key(s) & (a.block_size - 1));
+            mbar_expect_tx(&full[2 * to + which], own_half_bytes(D));
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
-            q[c] = live ? *reinterpret_cast<const uint4*>(qp + (c >> 1) * 128 + (c & 1) * 16) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    const int32_t* table = a.block_tables + static_cast<int64_t>(item.x) * a.max_blocks_per_seq;
-    auto first_key = [&](int s) { return prefix + s * kOwnStrip; };
-    auto page_of = [&](int s) { return s < s1 ? table[first_key(s) >> a.bs_log2] : 0; };
-    uint8_t* ring = smem + warp * ST * own_slot_bytes(D);
-    auto load = [&](int s, int blk, int slot) {     // (one lane)
-        uint8_t* dst = ring + slot * own_slot_bytes(D);
-        const int krow = (((blk * 2) * a.n_kv_heads + kvh) << a.bs_log2) + (first_key(s) & (a.block_size - 1));
-        const int vrow = krow + (a.n_kv_heads << a.bs_log2);
-        mbar_expect_tx(&full[warp][slot], own_slot_bytes(D));
-#pragma unroll
-        for (int c = 0; c < VC; ++c) tma_load_2d(dst + c * 2048, &tmap_kv, &full[warp][slot], c * 64, krow, kEvictFirst);
-#pragma unroll
-        for (int c = 0; c < VC; ++c) tma_load_2d(dst + (VC + c) * 2048, &tmap_kv, &full[warp][slot], c * 64, vrow, kEvictFirst);
-    };
-    float m_run = -INFINITY, l_run = 0.0f;
-    float acc[VC][8][4];
-#pragma unroll
-    for (int c = 0; c < VC; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[c][j][i] = 0.0f;
-
-    int next_page = 0;
-    if (lane == 0) {
-        int pages[ST];
-#pragma unroll
-        for (int i = 0; i < ST; ++i) pages[i] = page_of(s0 + i * W);
-#pragma unroll
-        for (int i = 0; i < ST; ++i)
-            if (s0 + i * W < s1) load(s0 + i * W, pages[i], i);
-        next_page = page_of(s0 + ST * W);
-    }
-    int slot = 0;
-    uint32_t phase = 0;
-    for (int s = s0; s < s1; s += W) {
-        const uint8_t* strip = ring + slot * own_slot_bytes(D);
-        const int key0 = first_key(s);
-        mbar_wait(&full[warp][slot], phase);
-        // ---- scores of 16 keys: two chains per tile of 8 ----
-        float sc[2][4], sd[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[i][e] = sd[i][e] = 0.0f;
-        }
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 k = *reinterpret_cast<const uint4*>(strip + (c >> 1) * 2048 + (g + 8 * i) * 128 + (((2 * t + (c & 1)) ^ g) << 4));
-                mma_m16n8k16<kBf16>(sc[i], q[c].x, 0u, q[c].y, 0u, k.x, k.y);
-                mma_m16n8k16<kBf16>(sd[i], q[c].z, 0u, q[c].w, 0u, k.z, k.w);
-            }
-        // ---- weights ----
-        float p[4];
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int pos = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
-            p[i] = live && pos <= q_pos ? (sc[i >> 1][i & 1] + sd[i >> 1][i & 1]) * a.scale_log2 : -INFINITY;
-            mx = fmaxf(mx, p[i]);
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run, mx);
-        if (__any_sync(0xffffffffu, m_new > m_run)) {
-            const float scale = m_run == -INFINITY ? 0.0f : sp_ex2(m_run - m_new);
-            l_run *= scale;
-#pragma unroll
-            for (int c = 0; c < VC; ++c)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[c][j][e] *= scale;
-            m_run = m_new;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            p[i] = m_run == -INFINITY ? 0.0f : sp_ex2(p[i] - m_run);
-            l_run += p[i];
-        }
-        // ---- O += P V: rounded weights in rows 0..7, what the rounding left in rows 8..15 ----
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] *= kUp;
-        const uint32_t h0 = pack2<kBf16>(p[0], p[1]), h1 = pack2<kBf16>(p[2], p[3]);
-        const uint32_t r0 = pack2<kBf16>(p[0] - unpack_lo<kBf16>(h0), p[1] - unpack_hi<kBf16>(h0));
-        const uint32_t r1 = pack2<kBf16>(p[2] - unpack_lo<kBf16>(h1), p[3] - unpack_hi<kBf16>(h1));
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-            uint4 vr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-                vr[i] = *reinterpret_cast<const uint4*>(strip + (VC + c) * 2048 + key * 128 + ((g ^ (key & 7)) << 4));
-                // rows past the last key may hold anything: no weight of zero makes that finite
-                if (key0 + kOwnStrip > kv_len && key0 + key >= kv_len) vr[i] = make_uint4(0u, 0u, 0u, 0u);
-            }
-            const uint32_t w0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, w1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
-            const uint32_t w2[4] = {vr[2].x, vr[2].y, vr[2].z, vr[2].w}, w3[4] = {vr[3].x, vr[3].y, vr[3].z, vr[3].w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                mma_m16n8k16<kBf16>(acc[c][j], h0, r0, h1, r1, __byte_perm(w0[j >> 1], w1[j >> 1], sel), __byte_perm(w2[j >> 1], w3[j >> 1], sel));
-            }
-        }
-        __syncwarp();       // (the slot has been read)
+            for (int c = 0; c < VC; ++c) tma_load_2d(dst + c * 2048, &tmap_kv, &full[2 * to + which], c * 64, row, kEvictFirst);
+        };
+        int v_page = 0, k_page = 0;      // of the strips that V and K are asked for next
         if (lane == 0) {
-            const int sn = s + ST * W;
-            if (sn < s1) load(sn, next_page, slot);
-            next_page = page_of(sn + W);
+            int pages[ST];
+#pragma unroll
+            for (int i = 0; i < ST; ++i) pages[i] = page_of(s0 + i);
+#pragma unroll
+            for (int i = 0; i < ST; ++i) {
+                if (s0 + i >= s1) break;
+                load(s0 + i, pages[i], (n + i) % ST, 0);
+                load(s0 + i, pages[i], (n + i) % ST, 1);
+            }
+            v_page = page_of(s0 + ST);
+            k_page = page_of(s0 + ST + 1);
         }
-        if (++slot == ST) {
-            slot = 0;
-            phase ^= 1;
+        // ---- my query row, pieces of 8 dims permuted as K's are ----
+        const bool live = g < rows;
+        const int r_tok = live ? (first_row + g) / G : 0, r_head = kvh * G + (live ? (first_row + g) % G : 0);
+        const int q_pos = kv_len - item.z + r_tok;
+        uint4 q[KC];
+        {
+            const char* qp = reinterpret_cast<const char*>(a.q) + ((static_cast<int64_t>(item.y) + r_tok) * a.ld_q + r_head * D) * 2 + t * 32;
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+                q[c] = live ? *reinterpret_cast<const uint4*>(qp + (c >> 1) * 128 + (c & 1) * 16) : make_uint4(0u, 0u, 0u, 0u);
         }
-    }
-
-    // ---- the warps' states through shared memory: each in its own ring, whose loads have all been waited for ----
-    auto mg_o = [&](int w, int r) { return reinterpret_cast<float*>(smem + w * ST * own_slot_bytes(D)) + r * LD; };
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-    l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-    if (live) {
-        if (t == 0) {
-            mg_ml[warp][g][0] = m_run;
-            mg_ml[warp][g][1] = l_run;
-        }
+        float m_run = -INFINITY, l_run = 0.0f;
+        float acc[VC][8][4];
 #pragma unroll
         for (int c = 0; c < VC; ++c)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float4* d = reinterpret_cast<float4*>(mg_o(warp, g) + c * 64 + (2 * t + e) * 8);
-                auto sum = [&](int j) { return (acc[c][j][e] + acc[c][j][e + 2]) * (1.0f / kUp); };
-                d[0] = make_float4(sum(0), sum(1), sum(2), sum(3));
-                d[1] = make_float4(sum(4), sum(5), sum(6), sum(7));
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[c][j][i] = 0.0f;
+        // ---- scores of 16 keys: two chains per tile of 8 ----
+        float sc[2][4], sd[2][4];
+        auto products = [&](int slot) {
+            const uint8_t* strip = ring + 2 * slot * own_half_bytes(D);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[i][e] = sd[i][e] = 0.0f;
             }
-    }
-    __syncthreads();
-    if (a.has_prefix) pdl_enter();
-    // the prefix' parts join, and the row is finished
-    auto finish = [&](int r, int dd, OwnJoin& j) {
-        const int tok = (first_row + r) / G, head = kvh * G + (first_row + r) % G;
-        const int64_t row = item.y + tok;
-        const int64_t part = static_cast<int64_t>(a.rows) * a.n_q_heads, place = row * a.n_q_heads + head;
-        for (int sp = 0; prefix > 0 && sp < 2 * a.p_splits; sp += 8) {        // eight parts' loads at once
-            float2 ml[8];
-            float4 x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ml[i] = sp + i < 2 * a.p_splits ? __ldcg(reinterpret_cast<const float2*>(a.ws_ml + ((sp + i) * part + place) * 2)) : make_float2(-INFINITY, 0.0f);
+            for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (ml[i].x != -INFINITY) x[i] = __ldcg(reinterpret_cast<const float4*>(a.ws_o + ((sp + i) * part + place) * D + dd));
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 k = *reinterpret_cast<const uint4*>(strip + (c >> 1) * 2048 + (g + 8 * i) * 128 + (((2 * t + (c & 1)) ^ g) << 4));
+                    mma_m16n8k16<kBf16>(sc[i], q[c].x, 0u, q[c].y, 0u, k.x, k.y);
+                    mma_m16n8k16<kBf16>(sd[i], q[c].z, 0u, q[c].w, 0u, k.z, k.w);
+                }
+        };
+        mbar_wait(&full[2 * (n % ST)], (n / ST) & 1);
+        products(n % ST);
+        __syncwarp();
+        if (lane == 0 && s0 + ST < s1) load(s0 + ST, v_page, n % ST, 0);
+        for (int s = s0; s < s1; ++s, ++n) {
+            const int slot = n % ST, ahead = (n + 1) % ST;
+            const uint8_t* strip = ring + (2 * slot + 1) * own_half_bytes(D);
+            const int key0 = first_key(s);
+            // ---- weights ----
+            float p[4];
+            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) j.add(ml[i].x, ml[i].y, x[i]);
+            for (int i = 0; i < 4; ++i) {
+                const int pos = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
+                p[i] = live && pos <= q_pos ? (sc[i >> 1][i & 1] + sd[i >> 1][i & 1]) * a.scale_log2 : -INFINITY;
+                mx = fmaxf(mx, p[i]);
+            }
+            // (the next strip's scores meanwhile; behind the last one a product of anything, which nothing uses)
+            if (s + 1 < s1) mbar_wait(&full[2 * ahead], ((n + 1) / ST) & 1);
+            products(ahead);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m_run, mx);
+            if (__any_sync(0xffffffffu, m_new > m_run)) {
+                const float scale = m_run == -INFINITY ? 0.0f : sp_ex2(m_run - m_new);
+                l_run *= scale;
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[c][j][e] *= scale;
+                m_run = m_new;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = m_run == -INFINITY ? 0.0f : sp_ex2(p[i] - m_run);
+                l_run += p[i];
+            }
+            // ---- O += P V: rounded weights in rows 0..7, what the rounding left in rows 8..15 ----
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] *= kUp;
+            const uint32_t h0 = pack2<kBf16>(p[0], p[1]), h1 = pack2<kBf16>(p[2], p[3]);
+            const uint32_t r0 = pack2<kBf16>(p[0] - unpack_lo<kBf16>(h0), p[1] - unpack_hi<kBf16>(h0));
+            const uint32_t r1 = pack2<kBf16>(p[2] - unpack_lo<kBf16>(h1), p[3] - unpack_hi<kBf16>(h1));
+            mbar_wait(&full[2 * slot + 1], (n / ST) & 1);
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                uint4 vr[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+                    vr[i] = *reinterpret_cast<const uint4*>(strip + c * 2048 + key * 128 + ((g ^ (key & 7)) << 4));
+                    // rows past the last key may hold anything: no weight of zero makes that finite
+                    if (key0 + kOwnStrip > kv_len && key0 + key >= kv_len) vr[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                const uint32_t w0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w}, w1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+                const uint32_t w2[4] = {vr[2].x, vr[2].y, vr[2].z, vr[2].w}, w3[4] = {vr[3].x, vr[3].y, vr[3].z, vr[3].w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                    mma_m16n8k16<kBf16>(acc[c][j], h0, r0, h1, r1, __byte_perm(w0[j >> 1], w1[j >> 1], sel), __byte_perm(w2[j >> 1], w3[j >> 1], sel));
+                }
+            }
+            __syncwarp();       // (V of this strip and K of the next one have been read)
+            if (lane == 0) {
+                if (s + ST < s1) load(s + ST, v_page, slot, 1);
+                if (s + ST + 1 < s1) load(s + ST + 1, k_page, ahead, 0);
+                v_page = k_page;
+                k_page = page_of(s + ST + 2);
+            }
         }
-        uint2 v;
-        v.x = pack2<kBf16>(j.o[0] / j.l, j.o[1] / j.l);
-        v.y = pack2<kBf16>(j.o[2] / j.l, j.o[3] / j.l);
-        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + row * a.ld_out + head * D + dd) = v;
-    };
-    for (int e = tid; e < rows * (D / 4); e += W * 32) {
-        const int r = e / (D / 4), dd = (e % (D / 4)) * 4;
-        OwnJoin j;
+        // ---- my share of the unit to scratch ----
+        l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+        l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+        if (live) {
+            const int64_t at = static_cast<int64_t>(more.y + job.y + worker) * kOwnRows + g;
+            if (t == 0) *reinterpret_cast<float2*>(a.own_ml + at * 2) = make_float2(m_run, l_run);
 #pragma unroll
-        for (int w = 0; w < W; ++w) j.add(mg_ml[w][r][0], mg_ml[w][r][1], *reinterpret_cast<const float4*>(mg_o(w, r) + dd));
-        if (splits == 1) {
-            finish(r, dd, j);
-        } else {
-            *reinterpret_cast<float4*>(&cta_o[r][dd]) = make_float4(j.o[0], j.o[1], j.o[2], j.o[3]);
-            if (dd == 0) *reinterpret_cast<float2*>(cta_ml[r]) = make_float2(j.m, j.l);
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = (acc[c][j][e] + acc[c][j][e + 2]) * (1.0f / kUp);
+                    st_v8_f32(a.own_o + at * D + c * 64 + (2 * t + e) * 8, v);
+                }
+        }
+        // ---- the next unit: of this item, or the first one of the next item that has any ----
+        job.w -= s1 - s0;
+        job.z = 0;
+        if (++job.y == a.n_kv_heads * row_tiles && job.w > 0) {
+            job.y = 0;
+            do ++job.x;
+            while (a.items[2 * job.x + 1].z == 0);
         }
     }
-    if (splits == 1) return;
-    own_cluster_sync();
-    for (int e = tid + static_cast<int>(own_cluster_rank()) * W * 32; e < rows * (D / 4); e += splits * W * 32) {
-        const int r = e / (D / 4), dd = (e % (D / 4)) * 4;
-        OwnJoin j;
-        for (int c = 0; c < splits; ++c) {
-            const float2 ml = own_load2(cta_ml[r], c);
-            j.add(ml.x, ml.y, own_load4(&cta_o[r][dd], c));
-        }
-        finish(r, dd, j);
-    }
-    own_cluster_sync();       // nobody leaves while its sums are read
 }
 
 template <int D, bool kBf16>
-static int launch_shared(const CUtensorMap& tq, const CUtensorMap& tkv, const CUtensorMap& tstrip, const SharedArgs& a, int n_tiles, int n_items,
-                         int o_splits, cudaStream_t s) {
-    auto pre = shared_prefix_kernel<D, kBf16>;
-    auto own = shared_own_kernel<D, kBf16>;
+__global__ void __launch_bounds__(kSpThreads, 1)
+shared_parts_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ CUtensorMap tmap_strip,
+                    const SharedArgs a) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    pdl_enter();
+    const int own_ctas = (a.n_workers + kOwnWarps - 1) / kOwnWarps;
+    if (static_cast<int>(blockIdx.x) >= own_ctas) shared_prefix<D, kBf16>(tmap_q, tmap_kv, a, smem, blockIdx.x - own_ctas);
+    else shared_own<D, kBf16>(tmap_strip, a, smem, blockIdx.x * kOwnWarps + (threadIdx.x >> 5));
+}
+
+// ---- the end -------------------------------------------------------------------------------------------------------------
+// A row of one head has D / 4 lanes, four outputs each, or `share` times as many where rows are few: then these share out its parts. The lanes of a
+// share hold the weights of the parts lane, lane + D / 4, ... of it; then all of them add up the outputs of its parts, eight parts' loads at once.
+constexpr int kJoinThreads = 128;
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kJoinThreads, 6) shared_join_kernel(const SharedArgs a, int share) {
+    constexpr int L = D / 4;
+    constexpr int KEEP = 160 / L;          // weights per lane: of 160 parts at a time
+    __shared__ float4 other_o[kJoinThreads];
+    __shared__ float2 other_ml[kJoinThreads];
+    const int lane = threadIdx.x % L, dd = lane * 4, group = threadIdx.x / L, mine = group % share;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * (kJoinThreads / L / share) + group / share;
+    const int row = static_cast<int>(min(i / a.n_q_heads, static_cast<int64_t>(a.rows) - 1)), head = static_cast<int>(i % a.n_q_heads);
+    const bool in = i < static_cast<int64_t>(a.rows) * a.n_q_heads;
+    // (the plan: no kernel writes it)
+    const int G = a.n_q_heads / a.n_kv_heads, it = a.row_items[row];
+    const int4 item = a.items[2 * it], more = a.items[2 * it + 1];
+    const int r = (row - item.y) * G + head % G, unit = more.y + head / G * more.z + r / kOwnRows;
+    const int2 workers = a.units[unit];
+    const int n_own = workers.y - workers.x + 1, n_pre = more.x > 0 ? 2 * a.p_splits : 0, n = n_pre + n_own;
+    const int64_t part = static_cast<int64_t>(a.rows) * a.n_q_heads, place = static_cast<int64_t>(row) * a.n_q_heads + head;
+    const int n_mine = (n - mine + share - 1) / share;       // parts mine, mine + share, ...
+    auto at = [&](int k) { return k < n_pre ? k * part + place : static_cast<int64_t>(unit + workers.x + k - n_pre) * kOwnRows + r % kOwnRows; };
+    pdl_enter();
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // (all lanes of a warp together, here and below: its rows and shares may have different numbers of parts)
+    for (int k0 = 0; __any_sync(0xffffffffu, k0 < n_mine); k0 += KEEP * L) {
+        float2 ml[KEEP];
+        float mx = m;
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) {
+            const int j = k0 + q * L + lane, k = mine + j * share;
+            ml[q] = j < n_mine ? __ldcg(reinterpret_cast<const float2*>((k < n_pre ? a.ws_ml : a.own_ml) + at(k) * 2)) : make_float2(-INFINITY, 0.0f);
+            mx = fmaxf(mx, ml[q].x);
+        }
+#pragma unroll
+        for (int s = L / 2; s > 0; s >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
+        const float old = m == -INFINITY ? 0.0f : sp_ex2(m - mx);
+        l *= old;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= old;
+        m = mx;
+        float sum = 0.0f;
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) {
+            ml[q].x = ml[q].x == -INFINITY ? 0.0f : sp_ex2(ml[q].x - mx);
+            sum = fmaf(ml[q].x, ml[q].y, sum);
+        }
+#pragma unroll
+        for (int s = L / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        l += sum;
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) {
+            const int last = min(n_mine - k0 - q * L, L);
+            for (int c = 0; __any_sync(0xffffffffu, c < last); c += 8) {
+                float w[8];
+                float4 x[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    w[u] = __shfl_sync(0xffffffffu, ml[q].x, (c + u) % L, L);
+                    if (c + u >= last) w[u] = 0.0f;
+                    const int k = mine + (k0 + q * L + c + u) * share;       // (parts without weight may hold anything)
+                    x[u] = w[u] != 0.0f ? __ldcg(reinterpret_cast<const float4*>((k < n_pre ? a.ws_o : a.own_o) + at(k) * D + dd)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    o[0] = fmaf(w[u], x[u].x, o[0]);
+                    o[1] = fmaf(w[u], x[u].y, o[1]);
+                    o[2] = fmaf(w[u], x[u].z, o[2]);
+                    o[3] = fmaf(w[u], x[u].w, o[3]);
+                }
+            }
+        }
+    }
+    if (share > 1) {
+        other_ml[threadIdx.x] = make_float2(m, l);
+        other_o[threadIdx.x] = make_float4(o[0], o[1], o[2], o[3]);
+        __syncthreads();
+        if (mine > 0) return;
+        float mx = m;
+        for (int k = 1; k < share; ++k) mx = fmaxf(mx, other_ml[threadIdx.x + k * L].x);      // (finite: a row has its own key)
+        const float f = sp_ex2(m - mx);
+        l *= f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= f;
+        for (int k = 1; k < share; ++k) {
+            const float2 x = other_ml[threadIdx.x + k * L];
+            const float4 y = other_o[threadIdx.x + k * L];
+            const float w = sp_ex2(x.x - mx);
+            l = fmaf(w, x.y, l);
+            o[0] = fmaf(w, y.x, o[0]);
+            o[1] = fmaf(w, y.y, o[1]);
+            o[2] = fmaf(w, y.z, o[2]);
+            o[3] = fmaf(w, y.w, o[3]);
+        }
+    }
+    if (!in) return;
+    uint2 v;
+    v.x = pack2<kBf16>(o[0] / l, o[1] / l);
+    v.y = pack2<kBf16>(o[2] / l, o[3] / l);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + row * a.ld_out + head * D + dd) = v;
+}
+
+template <int D, bool kBf16>
+static int launch_shared(const CUtensorMap& tq, const CUtensorMap& tkv, const CUtensorMap& tstrip, const SharedArgs& a, cudaStream_t s) {
+    auto parts = shared_parts_kernel<D, kBf16>;
     static bool configured[64] = {false};
     int dev = 0;
     cudaGetDevice(&dev);
     if (!configured[dev & 63]) {
-        HDS_CHECK_CUDA(cudaFuncSetAttribute(pre, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sp_smem_bytes(D))));
-        HDS_CHECK_CUDA(cudaFuncSetAttribute(own, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem_bytes(D)));
+        HDS_CHECK_CUDA(cudaFuncSetAttribute(parts, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sp_smem_bytes(D))));
         configured[dev & 63] = true;
     }
-    if (n_tiles > 0) HDS_CHECK_CUDA(launch_kernel(pre, dim3(n_tiles, a.n_kv_heads, a.p_splits), dim3(kSpThreads), sp_smem_bytes(D), s, tq, tkv, a));
-    HDS_CHECK_CUDA(launch_kernel_cluster(own, o_splits, dim3(o_splits, n_items, a.n_kv_heads * a.row_tiles), dim3(kOwnWarps * 32), own_smem_bytes(D),
-                                         s, tstrip, a));
+    const int ctas = a.prefix_ctas + (a.n_workers + kOwnWarps - 1) / kOwnWarps;
+    HDS_CHECK_CUDA(launch_kernel(parts, dim3(ctas), dim3(kSpThreads), sp_smem_bytes(D), s, tq, tkv, tstrip, a));
+    const int64_t threads = static_cast<int64_t>(a.rows) * a.n_q_heads * (D / 4);
+    // (as long as all CTAs find room at once: 6 per SM)
+    const int share = threads <= 148 * 6 * kJoinThreads / 4 ? 4 : threads <= 148 * 6 * kJoinThreads / 2 ? 2 : 1;
+    HDS_CHECK_CUDA(launch_kernel(shared_join_kernel<D, kBf16>, dim3(static_cast<unsigned>((threads * share + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0,
+                                 s, a, share));
     return HDS_OK;
 }
 
@@ -673,51 +717,66 @@ static int launch_shared(const CUtensorMap& tq, const CUtensorMap& tkv, const CU
 
 using namespace hds;
 
-extern "C" int64_t hds_paged_attention_shared_workspace_bytes(int rows, int n_q_heads, int head_dim, int p_splits) {
-    return static_cast<int64_t>(rows) * n_q_heads * (head_dim + 2) * 4 * 2 * p_splits;
+static int64_t shared_part_floats(int rows, int n_q_heads, int head_dim, int p_splits) {
+    return static_cast<int64_t>(rows) * n_q_heads * (head_dim + 2) * 2 * p_splits;
+}
+
+extern "C" int64_t hds_paged_attention_shared_workspace_bytes(int rows, int n_q_heads, int head_dim, int n_tiles, int p_splits, int n_units, int n_workers) {
+    return 4 * ((n_tiles > 0 ? shared_part_floats(rows, n_q_heads, head_dim, p_splits) : 0) +
+                (static_cast<int64_t>(n_units) + n_workers) * kOwnRows * (head_dim + 2));
 }
 
 extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out, int64_t ld_out, int rows, const void* kv_cache_layer,
                                           int64_t num_blocks, const int32_t* block_tables, int max_blocks_per_seq, const int32_t* tiles, int n_tiles,
-                                          int p_splits, const int32_t* items, int n_items, int max_tokens, int o_splits, int n_q_heads, int n_kv_heads,
-                                          int head_dim, int block_size, float scale, void* workspace, int64_t workspace_bytes, int dtype,
-                                          void* stream) {
+                                          int p_splits, const int32_t* items, const int32_t* workers, int n_workers, const int32_t* units, int n_units,
+                                          const int32_t* row_items, int n_q_heads, int n_kv_heads, int head_dim, int block_size, float scale,
+                                          void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
     HDS_REQUIRE(head_dim == 64 || head_dim == 128, "paged_attention_shared: head_dim must be 64 or 128");
     HDS_REQUIRE(block_size == 16 || block_size == 32 || block_size == 64 || block_size == 128, "paged_attention_shared: block_size must be 16/32/64/128");
     HDS_REQUIRE(n_kv_heads > 0 && n_q_heads > 0 && n_q_heads % n_kv_heads == 0 && n_q_heads / n_kv_heads <= 128,
                 "paged_attention_shared: up to 128 query heads per KV head");
     HDS_REQUIRE(dtype == 0 || dtype == 1, "paged_attention_shared: dtype must be 0 (bf16) or 1 (fp16)");
-    HDS_REQUIRE(p_splits >= 1 && p_splits <= 64 && (o_splits == 1 || o_splits == 2 || o_splits == 4 || o_splits == 8),
-                "paged_attention_shared: 1 to 64 splits of the prefix, 1, 2, 4 or 8 of a sequence's own keys");
-    HDS_REQUIRE(n_tiles >= 0 && n_items >= 0 && n_items <= 65535 && rows >= 0 && max_tokens >= 0, "paged_attention_shared: at most 65535 sequences");
-    if (n_items == 0 || rows == 0 || max_tokens == 0) return HDS_OK;
+    HDS_REQUIRE(p_splits >= 1 && p_splits <= 64, "paged_attention_shared: 1 to 64 splits of the prefix");
+    HDS_REQUIRE(n_tiles >= 0 && rows >= 0 && n_workers >= 0 && n_units >= 0, "paged_attention_shared: negative size");
+    if (rows == 0 || n_workers == 0) return HDS_OK;
     HDS_REQUIRE(ld_q % 8 == 0 && ld_out % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
                 "paged_attention_shared: rows start on 16-byte boundaries");
-    HDS_REQUIRE((reinterpret_cast<uintptr_t>(tiles) & 15) == 0 && (reinterpret_cast<uintptr_t>(items) & 15) == 0, "paged_attention_shared: unaligned work list");
+    HDS_REQUIRE(((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(items) | reinterpret_cast<uintptr_t>(workers)) & 15) == 0 &&
+                    (reinterpret_cast<uintptr_t>(units) & 7) == 0,
+                "paged_attention_shared: unaligned work lists");
     const int64_t kv_rows = num_blocks * 2 * n_kv_heads * block_size;
     HDS_REQUIRE(num_blocks > 0 && kv_rows < (int64_t(1) << 31), "paged_attention_shared: a layer's cache has fewer than 2^31 page rows");
+    HDS_REQUIRE(static_cast<int64_t>(n_tiles) * n_kv_heads * p_splits < (1 << 30) && static_cast<int64_t>(n_units) + n_workers < (1 << 30) &&
+                    static_cast<int64_t>(rows) * n_q_heads * (head_dim / 4) < (int64_t(1) << 38),
+                "paged_attention_shared: too much work for one call");
+    HDS_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 31) == 0 &&
+                    workspace_bytes >= hds_paged_attention_shared_workspace_bytes(rows, n_q_heads, head_dim, n_tiles, p_splits, n_units, n_workers),
+                "paged_attention_shared: workspace too small");
     const int G = n_q_heads / n_kv_heads;
     SharedArgs a;
     memset(&a, 0, sizeof(a));
-    a.row_tiles = static_cast<int>((static_cast<int64_t>(max_tokens) * G + kOwnRows - 1) / kOwnRows);
-    HDS_REQUIRE(static_cast<int64_t>(a.row_tiles) * n_kv_heads <= 65535, "paged_attention_shared: too many new tokens in a sequence");
-    HDS_REQUIRE(n_tiles == 0 || (workspace != nullptr && workspace_bytes >= hds_paged_attention_shared_workspace_bytes(rows, n_q_heads, head_dim, p_splits) &&
-                                 (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
-                "paged_attention_shared: workspace too small");
     a.q = q; a.out = out; a.ld_q = ld_q; a.ld_out = ld_out;
     a.block_tables = block_tables; a.max_blocks_per_seq = max_blocks_per_seq;
     a.tiles = reinterpret_cast<const int4*>(tiles);
     a.items = reinterpret_cast<const int4*>(items);
+    a.workers = reinterpret_cast<const int4*>(workers);
+    a.units = reinterpret_cast<const int2*>(units);
+    a.row_items = row_items;
+    a.n_tiles = n_tiles; a.n_workers = n_workers; a.prefix_ctas = n_tiles * n_kv_heads * p_splits;
     a.rows = rows; a.n_q_heads = n_q_heads; a.n_kv_heads = n_kv_heads;
     a.block_size = block_size;
     a.bs_log2 = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
     a.num_rows_kv = static_cast<int>(kv_rows);
     a.tile_tokens = 128 / G;
     a.p_splits = p_splits;
-    a.has_prefix = n_tiles > 0;
     a.scale_log2 = scale * 1.4426950408889634f;
-    a.ws_o = reinterpret_cast<float*>(workspace);       // the outputs first: they want 16-byte boundaries
-    a.ws_ml = a.ws_o + static_cast<int64_t>(2 * p_splits) * rows * n_q_heads * head_dim;
+    // the outputs first: they want 32-byte boundaries
+    const int64_t parts = n_tiles > 0 ? static_cast<int64_t>(2 * p_splits) * rows * n_q_heads : 0;
+    const int64_t shares = (static_cast<int64_t>(n_units) + n_workers) * kOwnRows;
+    a.ws_o = reinterpret_cast<float*>(workspace);
+    a.own_o = a.ws_o + parts * head_dim;
+    a.ws_ml = a.own_o + shares * head_dim;
+    a.own_ml = a.ws_ml + parts * 2;
     CUtensorMap tq, tkv, tstrip;
     memset(&tq, 0, sizeof(tq));
     int rc;
@@ -732,9 +791,6 @@ extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out
     rc = make_tmap_2d_16b(&tstrip, kv_cache_layer, head_dim, static_cast<uint64_t>(kv_rows), static_cast<uint64_t>(head_dim) * 2, 64, kOwnStrip, dtype == 0);
     if (rc) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (head_dim == 128)
-        return dtype == 0 ? launch_shared<128, true>(tq, tkv, tstrip, a, n_tiles, n_items, o_splits, s)
-                          : launch_shared<128, false>(tq, tkv, tstrip, a, n_tiles, n_items, o_splits, s);
-    return dtype == 0 ? launch_shared<64, true>(tq, tkv, tstrip, a, n_tiles, n_items, o_splits, s)
-                      : launch_shared<64, false>(tq, tkv, tstrip, a, n_tiles, n_items, o_splits, s);
+    if (head_dim == 128) return dtype == 0 ? launch_shared<128, true>(tq, tkv, tstrip, a, s) : launch_shared<128, false>(tq, tkv, tstrip, a, s);
+    return dtype == 0 ? launch_shared<64, true>(tq, tkv, tstrip, a, s) : launch_shared<64, false>(tq, tkv, tstrip, a, s);
 }

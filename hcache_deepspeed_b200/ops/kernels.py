@@ -1089,16 +1089,15 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
         return out
     lib = native.cuda_lib()
     with _On(index):
-        ws, n_bytes = None, 0
-        if plan.n_tiles:      # of this call alone: a plan may be in use on several streams, and in graphs
-            n_bytes = int(lib.hds_paged_attention_shared_workspace_bytes(rows, H, d, plan.p_splits))
-            ws = q.new_empty(n_bytes // q.element_size())
+        n_bytes = lib.hds_paged_attention_shared_workspace_bytes(rows, H, d, plan.n_tiles, plan.p_splits, plan.n_units, plan.n_workers)
+        ws = q.new_empty(n_bytes // 2)       # of this call alone: a plan may be in use on several streams, and in graphs
         rc = lib.hds_paged_attention_shared(q.data_ptr(), ld_q, out.data_ptr(), ld_out, rows, kv_cache_layer.data_ptr(), blocks, block_tables.data_ptr(), ld_tables,
-                                            plan.tiles_ptr, plan.n_tiles, plan.p_splits, plan.items_ptr, plan.n_seqs, plan.max_tokens, plan.o_splits, H,
-                                            plan.n_kv_heads, d, plan.block_size, scale, _p(ws), n_bytes, dt, _raw_stream(index))
+                                            plan.tiles_ptr, plan.n_tiles, plan.p_splits, plan.items_ptr, plan.workers_ptr, plan.n_workers, plan.units_ptr,
+                                            plan.n_units, plan.rows_ptr, H, plan.n_kv_heads, d, plan.block_size, scale, ws.data_ptr(), n_bytes, dt,
+                                            _raw_stream(index))
     if rc:
         native.check(rc, "hds_paged_attention_shared")
-    _count(2 if plan.n_tiles else 1)
+    _count(2)
     return out
 
 

@@ -64,7 +64,7 @@ def _declare_cuda(lib: ctypes.CDLL, partial: bool = False) -> None:
         "hds_gemm_next_act_limit": [F],
         "hds_adapter_add": [P, L, P, L, P, P, P, I, I, I, I, I, P, P, I, I, P, L, P, L, I, P],
         "hds_adapter_parts": [I, I],
-        "hds_paged_attention_shared": [P, L, P, L, I, P, L, P, I, P, I, I, P, I, I, I, I, I, I, I, F, P, L, I, P],
+        "hds_paged_attention_shared": [P, L, P, L, I, P, L, P, I, P, I, I, P, P, I, P, I, P, I, I, I, I, F, P, L, I, P],
         "hds_logit_controls": [P, L, P, L, I, I, P, L, I, P, P, P, P, P, P, L, P, L, I, P, L, I, P, I, P],
         "hds_moe_table_route": [P, P, I, I, I, I, P, P, P, P, P],
         "hds_moe_combine": [P, L, P, P, P, L, P, L, I, I, I, I, I, P],
@@ -139,7 +139,7 @@ def _declare_cuda(lib: ctypes.CDLL, partial: bool = False) -> None:
     lib.hds_linear_attention_workspace_bytes.restype = c_int64
     lib.hds_retention_workspace_bytes.argtypes = [I, I, I, I, I]
     lib.hds_retention_workspace_bytes.restype = c_int64
-    lib.hds_paged_attention_shared_workspace_bytes.argtypes = [I, I, I, I]
+    lib.hds_paged_attention_shared_workspace_bytes.argtypes = [I] * 7
     lib.hds_paged_attention_shared_workspace_bytes.restype = c_int64
     lib.hds_moe_padded_rows.argtypes = [I, I, I]
     lib.hds_moe_padded_rows.restype = c_int64

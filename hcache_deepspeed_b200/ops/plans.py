@@ -9,6 +9,12 @@ from typing import Sequence, Tuple
 import numpy as np
 import torch
 
+#: query rows of a unit, and keys of a strip, of a shared prefix' own keys
+OWN_ROWS, OWN_STRIP = 8, 16
+#: workers of a CTA for own keys; what beginning and end of a unit take, in strips
+OWN_WORKERS, OWN_BEGIN = 12, 2
+#: microseconds: an SM's for a strip of own keys, a CTA's for 128 keys of a prefix under one and under two tiles of rows (measured, see attention_shared.cu)
+T_OWN, T_ONE, T_TWO = 0.17, 1.3, 2.9
 #: rows of a tile of the adapter kernels, and of the tiles that go through one kernel
 ADAPTER_ROWS, ADAPTER_FEW = 64, 16
 
@@ -91,37 +97,55 @@ class SharedPrefixPlan:
                 lo, hi = int(row0[first]), int(row0[first + n])
                 tiles += [(first, r, min(tile_tokens, hi - r), length) for r in range(lo, hi, tile_tokens)]
         self.prefix = prefix
-        self.max_tokens = int(new.max()) if new.size else 0
         #: pages that the longest sequence needs in its block table
         self.max_blocks = -(-int(kv.max()) // block_size) if kv.size else 0
-        live = new > 0
-        row_tiles = max(1, -(-self.max_tokens * (n_q_heads // n_kv_heads) // 8))
-        self.p_splits = pick_prefix_splits(len(tiles) * n_kv_heads, max((t[3] for t in tiles), default=0))
-        self.o_splits = pick_own_splits(int(live.sum()) * n_kv_heads * row_tiles, int((kv - prefix)[live].max()) if live.any() else 0)
+        G = n_q_heads // n_kv_heads
         self.n_tiles = len(tiles)
+        # units of own keys: (sequence, KV head, 8 query rows); all their strips of 16 keys in one line, cut into pieces of equal cost for the workers
+        row_tiles = -(-new * G // OWN_ROWS)
+        strips = np.where(new > 0, -(-(kv - prefix) // OWN_STRIP), 0)
+        per_item = row_tiles * n_kv_heads
+        unit0 = np.concatenate([[0], np.cumsum(per_item)])
+        of_item = np.repeat(np.arange(new.size), per_item)                     # a unit's sequence
+        ends = np.concatenate([[0], np.cumsum(strips[of_item])])               # strips ahead of a unit
+        self.n_units, total = int(unit0[-1]), int(ends[-1])
+        if total >= 1 << 31:
+            raise ValueError("too many keys for one call")
+        # a unit costs its strips and a beginning and end that take as long as OWN_BEGIN more
+        costs = np.concatenate([[0], np.cumsum(np.where(strips[of_item] > 0, strips[of_item] + OWN_BEGIN, 0))])
+        self.p_splits, ctas = pick_shares(self.n_tiles * n_kv_heads, max((t[3] for t in tiles), default=0),
+                                          any(t[2] > tile_tokens // 2 for t in tiles), int(costs[-1]))
+        self.n_workers = W = min(ctas * OWN_WORKERS, -(-total // 2))
+        cost = costs[-1] * np.arange(W + 1, dtype=np.int64) // max(W, 1)
+        unit = np.searchsorted(costs, cost[:-1], side="right") - 1
+        cuts = np.concatenate([ends[unit] + np.maximum(cost[:-1] - costs[unit] - OWN_BEGIN, 0), [total]])
+        unit = np.searchsorted(ends, cuts[:-1], side="right") - 1
+        workers = np.stack([of_item[unit], unit - unit0[of_item[unit]], cuts[:-1] - ends[unit], np.diff(cuts)], axis=1) if W else np.zeros((0, 4))
+        units = np.stack([np.searchsorted(cuts, ends[:-1], side="right") - 1, np.searchsorted(cuts, ends[1:], side="left") - 1], axis=1)
         items = np.zeros((new.size, 8), dtype=np.int32)
-        items[:, 0], items[:, 1], items[:, 2], items[:, 3], items[:, 4] = np.arange(new.size), row0[:-1], new, kv, prefix
-        self.items = items
+        items[:, 0], items[:, 1], items[:, 2], items[:, 3] = np.arange(new.size), row0[:-1], new, kv
+        items[:, 4], items[:, 5], items[:, 6] = prefix, unit0[:-1], row_tiles
+        self.items, self.workers, self.units = items, workers.astype(np.int32), units.astype(np.int32)
         self.device = None if device is None else torch.device(device)
-        #: device number (-1: not on a GPU) and device pointers of the prefix' work list and of the sequences'
-        self.index, self.tiles_ptr, self.items_ptr = -1, 0, 0
+        #: device number (-1: not on a GPU) and device pointers
+        self.index = -1
         if self.device is not None and self.device.type == "cuda":
-            self._dev = torch.from_numpy(np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), items.reshape(-1)])).to(self.device)
-            self.index, self.tiles_ptr = self._dev.get_device(), self._dev.data_ptr()
-            self.items_ptr = self.tiles_ptr + 16 * self.n_tiles
+            row_items = np.repeat(np.arange(new.size), new).astype(np.int32)
+            parts = [np.asarray(tiles, dtype=np.int32), items, self.workers, self.units, row_items]       # all but the last start on 16-byte boundaries
+            flat = [np.concatenate([p.reshape(-1), np.zeros(-p.size % 4, dtype=np.int32)]) for p in parts]
+            self._dev = torch.from_numpy(np.concatenate(flat)).to(self.device)
+            self.index = self._dev.get_device()
+            at = self._dev.data_ptr() + 4 * np.cumsum([0] + [f.size for f in flat])
+            self.tiles_ptr, self.items_ptr, self.workers_ptr, self.units_ptr, self.rows_ptr = at[:5].tolist()
 
 
-def pick_prefix_splits(units: int, prefix: int, sms: int = 148) -> int:
-    """Parts of a prefix of that many tokens, ``units`` CTAs wide: the fewest waves of SMs, a CTA's beginning and end counted as two tiles."""
+def pick_shares(units: int, prefix: int, two: bool, cost: int, sms: int = 148) -> Tuple[int, int]:
+    """Parts of a prefix of that many tokens, ``units`` CTAs wide, and the CTAs for own keys of that cost in strips: both begin together, on SMs of
+    their own, and the later end counts. Within 5% of the best of 90 pairs at each of ten batches, where other pairs took up to twice as long."""
     tiles = -(-prefix // 128)
     if units == 0 or tiles == 0:
-        return 1
-    return min(range(1, min(64, tiles) + 1), key=lambda s: (-(-units * s // sms) * (-(-tiles // s) + 2), s))
-
-
-def pick_own_splits(units: int, keys: int, sms: int = 148) -> int:
-    """CTAs in a cluster for a sequence's own keys: two CTAs per SM, as long as each has 128 keys (two strips per warp)."""
-    splits = 1
-    while splits < 8 and units * splits * 2 <= 2 * sms and keys >= 256 * splits:
-        splits *= 2
-    return splits
+        return 1, sms
+    parts, ctas = np.arange(1, min(64, tiles) + 1)[:, None], np.arange(1, sms)[None, :]
+    ends = np.maximum(-(-units * parts // (sms - ctas)) * (5.0 + (T_TWO if two else T_ONE) * -(-tiles // parts)), 4.0 + T_OWN * cost / ctas)
+    best = int((ends + 0.05 * parts).argmin())      # (a part more to join)
+    return best // (sms - 1) + 1, best % (sms - 1) + 1

@@ -544,15 +544,19 @@ int hds_adapter_add(const void* base, int64_t ld_base, const void* x, int64_t ld
 int hds_adapter_parts(int n_tiles, int width);
 
 /* Paged attention of a batch whose sequences share prefixes. q and out: rows of n_q_heads * head_dim values, ld_q / ld_out apart; a group of
- * neighbouring sequences reads its prefix once. tiles int32 [n_tiles][4] = (sequence whose table names the prefix' pages, first row, tokens <=
- * 2 * (128 / (n_q_heads / n_kv_heads)), prefix); items int32 [n_items][8] = (sequence, first row, new tokens, keys, prefix, 0, 0, 0): row t of them sees
- * the keys up to keys - new tokens + t. Prefixes are whole pages ahead of the new tokens. p_splits (up to 64): parts of a prefix, o_splits
- * (1 / 2 / 4 / 8): CTAs for a sequence's other keys. workspace: see below; nothing in it outlives the call. dtype 0 / 1. */
+ * neighbouring sequences reads its prefix once. Work lists (ops/plans.py makes them; no kernel that may still run writes them), G = n_q_heads /
+ * n_kv_heads: tiles int32 [n_tiles][4] = (sequence whose table names the prefix' pages, first row, tokens <= 2 * (128 / G), prefix), cut into p_splits
+ * (up to 64) parts of the prefix each; items int32 [sequences][8] = (sequence, first row, new tokens, keys, prefix, first unit, row tiles, 0): row t
+ * of them sees the keys up to keys - new tokens + t, row tiles = ceil(new tokens * G / 8), units = (sequence, KV head, row tile) in this order;
+ * workers int32 [n_workers][4] = (item, unit in it, first strip of 16 own keys in the unit, strips), consecutive pieces of the line of all
+ * units' strips; units int32 [n_units][2] = (first, last worker); row_items int32 [rows] = the item of a row. Prefixes are whole pages ahead of the new
+ * tokens. workspace: see below; nothing in it outlives the call. dtype 0 / 1. */
 int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out, int64_t ld_out, int rows, const void* kv_cache_layer, int64_t num_blocks,
                                const int32_t* block_tables, int max_blocks_per_seq, const int32_t* tiles, int n_tiles, int p_splits,
-                               const int32_t* items, int n_items, int max_tokens, int o_splits, int n_q_heads, int n_kv_heads, int head_dim,
-                               int block_size, float scale, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
-int64_t hds_paged_attention_shared_workspace_bytes(int rows, int n_q_heads, int head_dim, int p_splits);
+                               const int32_t* items, const int32_t* workers, int n_workers, const int32_t* units, int n_units,
+                               const int32_t* row_items, int n_q_heads, int n_kv_heads, int head_dim, int block_size, float scale, void* workspace,
+                               int64_t workspace_bytes, int dtype, void* stream);
+int64_t hds_paged_attention_shared_workspace_bytes(int rows, int n_q_heads, int head_dim, int n_tiles, int p_splits, int n_units, int n_workers);
 
 /* What requests lay on their logits [rows, vocab] (dtype 0 / 1 / 2), out likewise (may be logits). Of history [rows, ld_history] the first
  * min(history_len, capacity) tokens of a row count, the first prompt_len of them as its prompt: x = x > 0 ? x / repetition : x * repetition for

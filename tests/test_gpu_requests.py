@@ -212,6 +212,8 @@ SHARED = [
     ([1, 2], [600, 3000], [], 16, 4, 128, 64),                                       # nothing is shared
     ([1] * 3, [2, 2, 2], [(0, 3, 4096)], 71, 1, 64, 128),                             # one KV head for 71: a tile of one token
     ([1] * 130, [1] * 130, [(0, 130, 48)], 1, 1, 128, 16),
+    ([1] * 4, [16000, 3, 1, 40], [(1, 2, 64)], 1, 1, 64, 16),                         # many parts next to few
+    ([1] * 160, [8000] + [1 + 3 * i % 20 for i in range(159)], [], 32, 1, 64, 16),    # the same with more rows than fill the device
 ]
 
 
@@ -233,14 +235,14 @@ def test_attention_behind_a_shared_prefix(dtype, new, own, groups, H, kvh, d, bs
     assert (out[-2:] == 7).all()        # rows behind the last sequence
 
 
-@pytest.mark.parametrize("splits", [(1, 1), (3, 2), (8, 4), (64, 8)])
+@pytest.mark.parametrize("splits", [1, 2, 3, 8, 64])
 @pytest.mark.parametrize("dtype", HALF)
 def test_parts_of_prefix_and_own_keys_join(dtype, splits):
     torch.manual_seed(6)
     new, keys, groups = [1, 2, 1], [1100 + 5, 1100 + 900, 2], [(0, 2, 1088)]
     cache, tables = pages(keys, groups, 2, 128, 64, dtype)
     plan = K().SharedPrefixPlan(new, keys, groups, 8, 2, 128, 64, device="cuda")
-    plan.p_splits, plan.o_splits = splits
+    plan.p_splits = splits
     q = rand(4, 1024, dtype=dtype, std=3.0)
     out = K().paged_attention_shared(q, torch.empty_like(q), cache, tables, plan, 128**-0.5)
     check(out, *attention_exact(q, cache, tables, new, keys, [1088, 1088, 0], 8, 128**-0.5))

@@ -72,7 +72,7 @@ def test_banks_refuse_what_does_not_fit():
 # ---- attention behind shared prefixes ----------------------------------------------------------------------------------
 def test_prefix_plan_lists_rows_and_lengths():
     plan = plans.SharedPrefixPlan([1, 0, 3, 2], [40, 32, 70, 5], [(0, 3, 32)], 8, 2, 64, 16)
-    assert plan.rows == 6 and plan.max_blocks == 5 and plan.max_tokens == 3
+    assert plan.rows == 6 and plan.max_blocks == 5
     assert plan.items[:, :5].tolist() == [[0, 0, 1, 40, 32], [1, 1, 0, 32, 32], [2, 1, 3, 70, 32], [3, 4, 2, 5, 0]]
     assert plan.n_tiles == 1      # four rows of 8 / 2 heads share a tile of 128
     wide = plans.SharedPrefixPlan([40] * 3, [200] * 3, [(0, 3, 128)], 8, 2, 64, 16)
@@ -99,9 +99,39 @@ def test_prefix_plans_refuse_heads_and_blocks():
 
 @pytest.mark.parametrize("units,prefix", [(0, 0), (1, 16), (1, 128), (1, 65536), (8, 4096), (32, 4096), (148, 8192), (1000, 100000)])
 def test_splits_of_a_prefix_have_tiles(units, prefix):
-    s = plans.pick_prefix_splits(units, prefix)
-    assert 1 <= s <= max(1, min(64, -(-prefix // 128)))
-    assert plans.pick_own_splits(units, prefix) in (1, 2, 4, 8)
+    for two in (False, True):
+        for cost in (1, 300, 12288, 1 << 40):
+            splits, ctas = plans.pick_shares(units, prefix, two, cost)
+            assert 1 <= splits <= max(1, min(64, -(-prefix // 128))) and 1 <= ctas <= 148
+
+
+@pytest.mark.parametrize("new,keys,groups,H,kvh", [
+    ([1], [1], [], 1, 1), ([1, 0, 3, 2], [40, 32, 70, 5], [(0, 3, 32)], 8, 2), ([0, 0, 5], [0, 9, 5], [], 71, 1), ([0, 0], [3, 3], [], 4, 4), ([], [], [], 4, 4),
+    ([1 + i % 3 for i in range(50)], [100 + (37 * i) % 901 for i in range(50)], [(0, 20, 96), (30, 5, 64)], 20, 2), ([1] * 3, [40000, 7, 39000], [], 32, 32),
+    ([1] * 300, [1 + (i % 7 == 0) * 900 for i in range(300)], [], 4, 4), ([1] * 40, [4097 + i for i in range(40)], [(0, 40, 4096)], 32, 8)])
+def test_own_keys_are_dealt_out_whole(new, keys, groups, H, kvh):
+    """Walking every worker's piece as the kernel does: each strip of each unit once, and the units' lists name just the workers that were there."""
+    plan = plans.SharedPrefixPlan(new, keys, groups, H, kvh, 64, 16)
+    items, seen, shares = plan.items.tolist(), {}, set()
+    for w, (item, unit, strip, left) in enumerate(plan.workers.tolist()):
+        assert left >= 0
+        while left > 0:
+            _, _, n, k, prefix, unit0, row_tiles, _ = items[item]
+            assert n > 0 and 0 <= unit < row_tiles * kvh
+            strips = -(-(k - prefix) // 16)
+            for s in range(strip, min(strips, strip + left)):
+                assert seen.setdefault((unit0 + unit, s), w) == w
+            shares.add((unit0 + unit, w))
+            left -= min(strips, strip + left) - strip
+            strip, unit = 0, unit + 1
+            if unit == row_tiles * kvh and left > 0:
+                unit, item = 0, item + 1
+                while items[item][6] == 0:
+                    item += 1
+    want = {(u, s) for _, _, n, k, prefix, unit0, rt, _ in items for u in range(unit0, unit0 + rt * kvh) for s in range(-(-(k - prefix) // 16))}
+    assert set(seen) == want
+    assert shares == {(u, w) for u, (a, b) in enumerate(plan.units.tolist()) for w in range(a, b + 1)}
+    assert len({u + w for u, w in shares}) == len(shares) and max((u + w for u, w in shares), default=-1) < plan.n_units + plan.n_workers
 
 
 def test_attention_of_a_group_on_the_host_is_that_of_its_sequences():
