@@ -63,8 +63,8 @@ __device__ __forceinline__ void ad_store4(uint32_t at, const float4& v) {
 }
 __device__ __forceinline__ uint4 ad_zero() { return make_uint4(0u, 0u, 0u, 0u); }
 
-// h rows of 16-bit values: 8 more than the rank, so that the rows of a fragment lie in different banks
-__host__ __device__ constexpr int ad_pitch(int rank) { return (rank + 15) / 16 * 16 + 8; }
+// h rows of 16-bit values: an odd number of 16 values, so that four rows of a fragment lie in different banks
+__host__ __device__ constexpr int ad_pitch(int rank) { return ((rank + 15) / 16 | 1) * 16; }
 
 // (ld: values between rows, below 2^30)
 __device__ __forceinline__ const uint16_t* ad_row(const void* p, int row, int ld) {
@@ -438,6 +438,9 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_down_kernel(const Adapt
 __host__ __device__ constexpr int ad_base_stages(int rank) { return rank <= 32 ? 3 : 2; }      // so that two CTAs fit an SM up to rank 64
 __host__ __device__ constexpr int ad_up_smem_bytes(int rank) { return ad_base_stages(rank) * kAdRows * kAdCols * 2 + 2 * kAdRows * ad_pitch(rank) * 2; }
 
+// where 16 bytes of a row of base are: half of the rows have neighbouring four pieces exchanged, as a quarter of a warp reads four of each of two rows
+__device__ __forceinline__ int ad_base_piece(int row, int piece) { return piece ^ (row & 1) * 4; }
+
 template <int KS, int RANK, bool kBf16>
 __global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const AdapterArgs a) {
     extern __shared__ __align__(16) uint8_t ad_smem[];
@@ -472,7 +475,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const Adapter
     auto load = [&](int i) {        // base of group number i (always ends a group of copies, an empty one behind the last)
         const int n = n_first + i * n_step + lane * 8;
         if (n < a.outputs) {
-            const uint32_t to = smem + i % stages * (kAdRows * kAdCols * 2) + lane * 16;
+            const uint32_t to = smem + i % stages * (kAdRows * kAdCols * 2) + ad_base_piece(warp, lane) * 16;      // (r is odd where warp is)
             for (int r = warp; r < min(m_tiles * 16, tile.z); r += kAdWarps) ad_copy_async(to + r * kAdCols * 2, ad_row(a.base, rows[r], a.ld_base) + n, true);
         }
         ad_copies_end();
@@ -535,7 +538,7 @@ __global__ void __launch_bounds__(kAdThreads, 2) adapter_up_kernel(const Adapter
         else ad_copies_wait<1>();
         __syncthreads();            // the stage is there, and h
         uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + col;
-        const uint8_t* base = ad_smem + i % stages * (kAdRows * kAdCols * 2) + (warp * 32 + t * 8) * 2;
+        const uint8_t* base = ad_smem + i % stages * (kAdRows * kAdCols * 2) + ad_base_piece(g, warp * 4 + t) * 16;
 #pragma unroll
         for (int m = 0; m < kAdRows / 16; ++m) {
             if (m >= m_tiles) break;
