@@ -130,9 +130,6 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
     uint8_t* q_sm = smem;                       // [row tile][panel][128 x 64]
     uint8_t* ring = smem + (two ? 2 : 1) * TILE_BYTES;
     const int bs = a.block_size, bps = kSpTok / bs;
-    // places of K and V of a key tile in the producer's order: K0 K1 V0 K2 V1 ... (two row tiles: K1 is asked for behind K0's products only)
-    auto seq_k = [&](int t) { return t < 2 ? t : 2 * t - 1; };
-    auto seq_v = [&](int t) { return n_tiles == 1 ? 1 : t >= n_tiles - 1 ? 2 * n_tiles - 1 : 2 * t + 2; };
 
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&tmap_q);
@@ -184,6 +181,7 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
                     phase ^= 1;
                 }
             };
+            // K0 K1 V0 K2 V1 ... (two row tiles: K1 is asked for behind K0's products only)
             load(0, 0);
             if (n_tiles > 1) load(1, 0);
             for (int t = 0; t < n_tiles; ++t) {
@@ -193,9 +191,19 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
         }
     } else if (warp == 1) {
         if (lane == 0 && n_tiles > 0) {
-            auto wait_full = [&](int seq) { mbar_wait(&full[seq % slots], (seq / slots) & 1); };
-            auto issue_qk = [&](int h, int seq) {
-                const uint8_t* ktile = ring + (seq % slots) * TILE_BYTES;
+            int next = 0;                  // (tiles are used in the order in which they are loaded)
+            uint32_t phase = 0;
+            auto take = [&]() {            // the slot of the next tile, when it is there
+                const int slot = next;
+                mbar_wait(&full[slot], phase);
+                if (++next == slots) {
+                    next = 0;
+                    phase ^= 1;
+                }
+                return slot;
+            };
+            auto issue_qk = [&](int h, int slot) {
+                const uint8_t* ktile = ring + slot * TILE_BYTES;
                 const uint8_t* qtile = q_sm + (two ? h : 0) * TILE_BYTES;
 #pragma unroll
                 for (int p = 0; p < PANELS; ++p) {
@@ -206,57 +214,52 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
                 }
                 umma_commit(&s_full[h]);
             };
-            auto issue_pv = [&](int h, int seq, bool first) {
-                const uint8_t* vtile = ring + (seq % slots) * TILE_BYTES;
+            auto issue_pv = [&](int h, int slot, bool first) {
+                const uint64_t dv = make_desc_mnmajor_sw128(smem_u32(ring + slot * TILE_BYTES), PANEL_BYTES);
 #pragma unroll
-                for (int kk = 0; kk < kSpTok / 16; ++kk)
-                    umma_f16_ts(tmem_base + 256 + h * 128, tmem_base + h * 128 + kk * 8,
-                                make_desc_mnmajor_sw128(smem_u32(vtile + kk * 16 * 128), PANEL_BYTES), IDESC_PV, (!first || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < kSpTok / 16; ++kk)        // (16 rows of 128 bytes further: 128 units of 16 bytes)
+                    umma_f16_ts(tmem_base + 256 + h * 128, tmem_base + h * 128 + kk * 8, dv + 128 * kk, IDESC_PV, (!first || kk > 0) ? 1u : 0u);
             };
             mbar_wait(q_full, 0);
-            wait_full(0);
+            const int k0 = take();
             tc_fence_after();
-            issue_qk(0, 0);
+            issue_qk(0, k0);
             if (two) {
-                issue_qk(1, 0);
-                umma_commit(&empty[0]);
+                issue_qk(1, k0);
+                umma_commit(&empty[k0]);
                 for (int t = 0; t < n_tiles; ++t) {
                     const bool more = t + 1 < n_tiles;
-                    const int sv = seq_v(t), sk = seq_k(t + 1);
-                    if (more) wait_full(sk);
-                    wait_full(sv);
+                    const int sk = more ? take() : 0, sv = take();
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         mbar_wait(&p_full[h], t & 1);
                         tc_fence_after();
                         issue_pv(h, sv, t == 0);
-                        if (h == 1) umma_commit(&empty[sv % slots]);
+                        if (h == 1) umma_commit(&empty[sv]);
                         if (more) issue_qk(h, sk);
                         else umma_commit(&o_full[h]);
                     }
-                    if (more) umma_commit(&empty[sk % slots]);
+                    if (more) umma_commit(&empty[sk]);
                 }
             } else {
-                umma_commit(&empty[0]);
+                umma_commit(&empty[k0]);
                 if (n_tiles > 1) {
-                    wait_full(1);
+                    const int k1 = take();
                     tc_fence_after();
-                    issue_qk(1, 1);
-                    umma_commit(&empty[1 % slots]);
+                    issue_qk(1, k1);
+                    umma_commit(&empty[k1]);
                 }
                 for (int t = 0; t < n_tiles; ++t) {
-                    const int h = t & 1, sv = seq_v(t);
-                    wait_full(sv);
+                    const int h = t & 1, sv = take();
                     mbar_wait(&p_full[h], (t >> 1) & 1);
                     tc_fence_after();
                     issue_pv(h, sv, t < 2);
-                    umma_commit(&empty[sv % slots]);
+                    umma_commit(&empty[sv]);
                     if (t + 2 < n_tiles) {
-                        const int sk = seq_k(t + 2);
-                        wait_full(sk);
+                        const int sk = take();
                         tc_fence_after();
                         issue_qk(h, sk);
-                        umma_commit(&empty[sk % slots]);
+                        umma_commit(&empty[sk]);
                     } else {
                         umma_commit(&o_full[h]);
                     }
