@@ -103,7 +103,7 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
     constexpr int PANEL_BYTES = kSpTok * 128;
     constexpr int TILE_BYTES = PANELS * PANEL_BYTES;
     constexpr int MAX_SLOTS = sp_tiles(D) - 1;
-    constexpr uint32_t IDESC_QK = make_idesc_f16(128, kSpTok, kBf16, false, false);
+    constexpr uint32_t IDESC_QK = make_idesc_f16(128, kSpTok / 2, kBf16, false, false);
     constexpr uint32_t IDESC_PV = make_idesc_f16(128, D, kBf16, false, true);
     constexpr float kUpLog2 = kBf16 ? 0.0f : 7.0f;     // (2^8 of a stale maximum and these stay below fp16's 2^16)
 
@@ -111,11 +111,10 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
     uint64_t* q_full = bars;
     uint64_t* full = bars + 1;
     uint64_t* empty = full + MAX_SLOTS;
-    uint64_t* s_full = empty + MAX_SLOTS;    // [stream] S of a tile is there (and P V of the tile before is done)
-    uint64_t* p_full = s_full + 2;           // [stream] P is there (and O rescaled)
-    uint64_t* o_full = p_full + 2;           // [stream] the last P V is done
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
-    static_assert((1 + 2 * MAX_SLOTS + 6) * 8 + 4 <= 512, "barriers have room");
+    uint64_t* s_full = empty + MAX_SLOTS;    // [stream][half] P V of the tile before is done, and S of half a tile is there unless it was the last one
+    uint64_t* p_full = s_full + 4;           // [stream][half] P is there (and O rescaled)
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 4);
+    static_assert((1 + 2 * MAX_SLOTS + 8) * 8 + 4 <= 512, "barriers have room");
 
     const uint32_t warp = warp_id(), lane = lane_id();
     const int4 tile = a.tiles[block % a.n_tiles];
@@ -139,10 +138,9 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int h = 0; h < 2; ++h) {
-            mbar_init(&s_full[h], 1);
-            mbar_init(&p_full[h], 4);
-            mbar_init(&o_full[h], 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
         }
         fence_barrier_init();
     }
@@ -155,24 +153,30 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
+    // The whole warp walks a producer's and an issuer's schedule and one elected lane issues: under `lane == 0` each tcgen05.mma took 90 cycles to
+    // issue (64 sequences of 64 heads behind 8192 keys 44.6 us, 39.0 with the elected lane).
+    const bool leader = elect_one();
     if (warp == 0) {
-        if (lane == 0 && n_tiles > 0) {
+        if (n_tiles > 0) {
             // tile row = token * G + head in group; rows behind the last whole token of 128 are never written, nor stored
-            mbar_expect_tx(q_full, (two ? 2 : 1) * PANELS * a.tile_tokens * G * 128);
-            for (int q = 0; q < (two ? 2 : 1); ++q)
+            if (leader) {
+                mbar_expect_tx(q_full, (two ? 2 : 1) * PANELS * a.tile_tokens * G * 128);
+                for (int q = 0; q < (two ? 2 : 1); ++q)
 #pragma unroll
-                for (int p = 0; p < PANELS; ++p)
-                    tma_load_3d(q_sm + q * TILE_BYTES + p * PANEL_BYTES, &tmap_q, q_full, p * 64, kvh * G, tile.y + q * a.tile_tokens, kEvictFirst);
+                    for (int p = 0; p < PANELS; ++p)
+                        tma_load_3d(q_sm + q * TILE_BYTES + p * PANEL_BYTES, &tmap_q, q_full, p * 64, kvh * G, tile.y + q * a.tile_tokens, kEvictFirst);
+            }
             const int32_t* table = a.block_tables + static_cast<int64_t>(tile.x) * a.max_blocks_per_seq;
             const int n_blocks = prefix / bs;
             uint32_t slot = 0, phase = 0;
             auto load = [&](int t, int which) {
                 mbar_wait(&empty[slot], phase ^ 1);
                 uint8_t* dst = ring + slot * TILE_BYTES;
-                mbar_expect_tx(&full[slot], TILE_BYTES);
+                if (leader) mbar_expect_tx(&full[slot], TILE_BYTES);
                 for (int b = 0; b < bps; ++b) {
                     const int bi = (t0 + t) * bps + b;
                     const int row = bi < n_blocks ? ((table[bi] * 2 + which) * a.n_kv_heads + kvh) * bs : a.num_rows_kv;      // behind the cache: zeros
+                    if (!leader) continue;
 #pragma unroll
                     for (int p = 0; p < PANELS; ++p) tma_load_2d(dst + p * PANEL_BYTES + b * bs * 128, &tmap_kv, &full[slot], p * 64, row, kEvictNormal);
                 }
@@ -190,7 +194,10 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && n_tiles > 0) {
+        if (n_tiles > 0) {
+            auto commit = [&](uint64_t* bar) {
+                if (leader) umma_commit(bar);
+            };
             int next = 0;                  // (tiles are used in the order in which they are loaded)
             uint32_t phase = 0;
             auto take = [&]() {            // the slot of the next tile, when it is there
@@ -202,67 +209,70 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
                 }
                 return slot;
             };
-            auto issue_qk = [&](int h, int slot) {
-                const uint8_t* ktile = ring + slot * TILE_BYTES;
+            auto issue_qk = [&](int h, int half, int slot) {
+                const uint8_t* ktile = ring + slot * TILE_BYTES + half * (kSpTok / 2) * 128;
                 const uint8_t* qtile = q_sm + (two ? h : 0) * TILE_BYTES;
+                if (!leader) return;
 #pragma unroll
                 for (int p = 0; p < PANELS; ++p) {
                     const uint64_t dq = make_desc_kmajor_sw128(smem_u32(qtile + p * PANEL_BYTES));
                     const uint64_t dk = make_desc_kmajor_sw128(smem_u32(ktile + p * PANEL_BYTES));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_f16_ss(tmem_base + h * 128, dq + 2 * k, dk + 2 * k, IDESC_QK, (p > 0 || k > 0) ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k)
+                        umma_f16_ss(tmem_base + h * 128 + half * 64, dq + 2 * k, dk + 2 * k, IDESC_QK, (p > 0 || k > 0) ? 1u : 0u);
                 }
-                umma_commit(&s_full[h]);
             };
-            auto issue_pv = [&](int h, int slot, bool first) {
-                const uint64_t dv = make_desc_mnmajor_sw128(smem_u32(ring + slot * TILE_BYTES), PANEL_BYTES);
+            auto issue_pv = [&](int h, int half, int slot, bool first) {
+                const uint64_t dv = make_desc_mnmajor_sw128(smem_u32(ring + slot * TILE_BYTES + half * (kSpTok / 2) * 128), PANEL_BYTES);
+                if (!leader) return;
 #pragma unroll
-                for (int kk = 0; kk < kSpTok / 16; ++kk)        // (16 rows of 128 bytes further: 128 units of 16 bytes)
-                    umma_f16_ts(tmem_base + 256 + h * 128, tmem_base + h * 128 + kk * 8, dv + 128 * kk, IDESC_PV, (!first || kk > 0) ? 1u : 0u);
+                for (int kk = 0; kk < kSpTok / 32; ++kk)        // (16 rows of 128 bytes further: 128 units of 16 bytes)
+                    umma_f16_ts(tmem_base + 256 + h * 128, tmem_base + h * 128 + half * 64 + kk * 8, dv + 128 * kk, IDESC_PV, (!first || half > 0 || kk > 0) ? 1u : 0u);
+            };
+            // P V of half a tile and, if there is a tile behind it for the stream, the products of the same half of that
+            auto step = [&](int h, int half, int sv, bool first, uint32_t parity, int sk, bool more) {
+                mbar_wait(&p_full[2 * h + half], parity);
+                tc_fence_after();
+                issue_pv(h, half, sv, first);
+                if (more) issue_qk(h, half, sk);
+                commit(&s_full[2 * h + half]);
+            };
+            auto begin = [&](int h, int slot) {
+                for (int half = 0; half < 2; ++half) {
+                    issue_qk(h, half, slot);
+                    commit(&s_full[2 * h + half]);
+                }
             };
             mbar_wait(q_full, 0);
             const int k0 = take();
             tc_fence_after();
-            issue_qk(0, k0);
+            begin(0, k0);
             if (two) {
-                issue_qk(1, k0);
-                umma_commit(&empty[k0]);
+                begin(1, k0);
+                commit(&empty[k0]);
                 for (int t = 0; t < n_tiles; ++t) {
                     const bool more = t + 1 < n_tiles;
                     const int sk = more ? take() : 0, sv = take();
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        mbar_wait(&p_full[h], t & 1);
-                        tc_fence_after();
-                        issue_pv(h, sv, t == 0);
-                        if (h == 1) umma_commit(&empty[sv]);
-                        if (more) issue_qk(h, sk);
-                        else umma_commit(&o_full[h]);
-                    }
-                    if (more) umma_commit(&empty[sk]);
+#pragma unroll 1
+                    for (int i = 0; i < 4; ++i) step(i & 1, i >> 1, sv, t == 0, t & 1, sk, more);
+                    commit(&empty[sv]);
+                    if (more) commit(&empty[sk]);
                 }
             } else {
-                umma_commit(&empty[k0]);
+                commit(&empty[k0]);
                 if (n_tiles > 1) {
                     const int k1 = take();
                     tc_fence_after();
-                    issue_qk(1, k1);
-                    umma_commit(&empty[k1]);
+                    begin(1, k1);
+                    commit(&empty[k1]);
                 }
                 for (int t = 0; t < n_tiles; ++t) {
-                    const int h = t & 1, sv = take();
-                    mbar_wait(&p_full[h], (t >> 1) & 1);
-                    tc_fence_after();
-                    issue_pv(h, sv, t < 2);
-                    umma_commit(&empty[sv]);
-                    if (t + 2 < n_tiles) {
-                        const int sk = take();
-                        tc_fence_after();
-                        issue_qk(h, sk);
-                        umma_commit(&empty[sk]);
-                    } else {
-                        umma_commit(&o_full[h]);
-                    }
+                    const bool more = t + 2 < n_tiles;
+                    const int sv = take(), sk = more ? take() : 0;
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) step(t & 1, half, sv, t < 2, (t >> 1) & 1, sk, more);
+                    commit(&empty[sv]);
+                    if (more) commit(&empty[sk]);
                 }
             }
         }
@@ -275,30 +285,32 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
         const int live_rows = (two ? (h == 0 ? a.tile_tokens : tile.z - a.tile_tokens) : tile.z) * G;
         const bool quad_live = static_cast<int>(quad * 32) < live_rows;   // warp-uniform
         const int steps = two ? n_tiles : (n_tiles - h + 1) >> 1;
-        const uint32_t tmem_s = tmem_base + h * 128 + ((quad * 32u) << 16);
-        const uint32_t tmem_o = tmem_s + 256;
+        const uint32_t tmem_stream = tmem_base + h * 128 + ((quad * 32u) << 16);
+        const uint32_t tmem_o = tmem_stream + 256;
         constexpr float kRescaleThreshold = 8.0f;
         float m_run = -INFINITY, l_run = 0.0f;       // m_run in log2 units, kUpLog2 not in it
-        for (int i = 0; i < steps; ++i) {
-            mbar_wait(&s_full[h], i & 1);
+        for (int i = 0; i < 2 * steps; ++i) {        // half a tile at a time: while one half is weighed, the other one's products run
+            const int half = i & 1;
+            const uint32_t tmem_s = tmem_stream + half * 64;
+            mbar_wait(&s_full[2 * h + half], (i >> 1) & 1);
             tc_fence_after();
             if (!quad_live) {
-                if (lane == 0) mbar_arrive(&p_full[h]);
+                if (lane == 0) mbar_arrive(&p_full[2 * h + half]);
                 continue;
             }
-            const int left = prefix - (t0 + (two ? i : 2 * i + h)) * kSpTok;      // keys from the tile's first on
-            uint32_t sr[128];
+            const int left = prefix - (t0 + (two ? i >> 1 : (i & ~1) + h)) * kSpTok - half * 64;      // keys from the half's first on
+            uint32_t sr[64];
 #pragma unroll
-            for (int c = 0; c < 128; c += 32) tmem_ld_32x32(tmem_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sr[c]));
+            for (int c = 0; c < 64; c += 32) tmem_ld_32x32(tmem_s + c, *reinterpret_cast<uint32_t(*)[32]>(&sr[c]));
             tmem_ld_wait();
-            if (left < kSpTok) {
+            if (left < 64) {
 #pragma unroll
-                for (int j = 0; j < 128; ++j)
+                for (int j = 0; j < 64; ++j)
                     if (j >= left) sr[j] = __float_as_uint(-INFINITY);
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 128; j += 8)
+            for (int j = 0; j < 64; j += 8)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) mx[q] = fmaxf(mx[q], fmaxf(__uint_as_float(sr[j + 2 * q]), __uint_as_float(sr[j + 2 * q + 1])));
             const float tmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
@@ -309,7 +321,9 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
             const float alpha = (!grow || fresh) ? (grow ? 0.0f : 1.0f) : sp_ex2(m_run - m_new);
             const float m_sub = ((m_new == -INFINITY) ? 0.0f : m_new) - kUpLog2;
             m_run = m_new;
-            if (i > 0 && __any_sync(0xffffffffu, grow && !fresh)) {     // (S has arrived: P V of the tile before is done)
+            if (i > 0 && __any_sync(0xffffffffu, grow && !fresh)) {
+                mbar_wait(&s_full[2 * h + (half ^ 1)], ((i + 1) >> 1) & 1);     // P V of the half before is done
+                tc_fence_after();
                 const float f = grow && !fresh ? alpha : 1.0f;
 #pragma unroll
                 for (int c = 0; c < D; c += 16) {
@@ -323,27 +337,24 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
             }
             const uint64_t k2 = sp_pack(a.scale_log2, a.scale_log2), m2 = sp_pack(-m_sub, -m_sub);
             uint64_t sum[2] = {0ull, 0ull};
+            uint32_t packed[32];
 #pragma unroll
-            for (int c = 0; c < 128; c += 64) {
-                uint32_t packed[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float x0, x1;
-                    sp_unpack(sp_fma(sp_pack(__uint_as_float(sr[c + 2 * j]), __uint_as_float(sr[c + 2 * j + 1])), k2, m2), x0, x1);
-                    x0 = sp_ex2(x0);
-                    x1 = sp_ex2(x1);
-                    sum[j & 1] = sp_add(sum[j & 1], sp_pack(x0, x1));
-                    packed[j] = pack2<kBf16>(x0, x1);
-                }
-                tmem_st_32x32(tmem_s + c / 2, packed);
+            for (int j = 0; j < 32; ++j) {
+                float x0, x1;
+                sp_unpack(sp_fma(sp_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), k2, m2), x0, x1);
+                x0 = sp_ex2(x0);
+                x1 = sp_ex2(x1);
+                sum[j & 1] = sp_add(sum[j & 1], sp_pack(x0, x1));
+                packed[j] = pack2<kBf16>(x0, x1);
             }
+            tmem_st_32x32(tmem_s, packed);
             float u0, u1;
             sp_unpack(sp_add(sum[0], sum[1]), u0, u1);
             l_run = l_run * alpha + (u0 + u1);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[h]);
+            if (lane == 0) mbar_arrive(&p_full[2 * h + half]);
         }
         // ---- parts: number `split` and, of the second key stream, p_splits + split (nothing in it with two row tiles) ----
         const int tok = r / G;
@@ -355,7 +366,7 @@ __device__ __forceinline__ void shared_prefix(const CUtensorMap& tmap_q, const C
             if (two) *reinterpret_cast<float2*>(a.ws_ml + ((a.p_splits + split) * part + place) * 2) = make_float2(-INFINITY, 0.0f);
         }
         if (steps > 0) {
-            mbar_wait(&o_full[h], 0);
+            for (int half = 0; half < 2; ++half) mbar_wait(&s_full[2 * h + half], steps & 1);
             tc_fence_after();
             if (quad_live) {
 #pragma unroll
@@ -410,6 +421,7 @@ __device__ __forceinline__ void shared_own(const CUtensorMap& tmap_kv, const Sha
         fence_barrier_init();
     }
     __syncwarp();
+    const bool leader = elect_one();
     const int G = a.n_q_heads / a.n_kv_heads;
     int n = 0;                           // strips so far: strip n has slot n % ST
     int4 job = a.workers[worker];        // (item, unit in the item, first strip in the unit, strips)
@@ -423,7 +435,7 @@ __device__ __forceinline__ void shared_own(const CUtensorMap& tmap_kv, const Sha
         const int32_t* table = a.block_tables + static_cast<int64_t>(item.x) * a.max_blocks_per_seq;
         auto first_key = [&](int s) { return prefix + s * kOwnStrip; };
         auto page_of = [&](int s) { return s < s1 ? table[first_key(s) >> a.bs_log2] : 0; };
-        auto load = [&](int s, int blk, int to, int which) {     // (one lane)
+        auto load = [&](int s, int blk, int to, int which) {     // (the elected lane)
             uint8_t* dst = ring + (2 * to + which) * own_half_bytes(D);
             const int row = (((blk * 2 + which) * a.n_kv_heads + kvh) << a.bs_log2) + (first_key(s) & (a.block_size - 1));
             mbar_expect_tx(&full[2 * to + which], own_half_bytes(D));
@@ -431,13 +443,13 @@ __device__ __forceinline__ void shared_own(const CUtensorMap& tmap_kv, const Sha
             for (int c = 0; c < VC; ++c) tma_load_2d(dst + c * 2048, &tmap_kv, &full[2 * to + which], c * 64, row, kEvictFirst);
         };
         int v_page = 0, k_page = 0;      // of the strips that V and K are asked for next
-        if (lane == 0) {
+        {
             int pages[ST];
 #pragma unroll
             for (int i = 0; i < ST; ++i) pages[i] = page_of(s0 + i);
 #pragma unroll
             for (int i = 0; i < ST; ++i) {
-                if (s0 + i >= s1) break;
+                if (s0 + i >= s1 || !leader) break;
                 load(s0 + i, pages[i], (n + i) % ST, 0);
                 load(s0 + i, pages[i], (n + i) % ST, 1);
             }
@@ -484,7 +496,7 @@ __device__ __forceinline__ void shared_own(const CUtensorMap& tmap_kv, const Sha
         mbar_wait(&full[2 * (n % ST)], (n / ST) & 1);
         products(n % ST);
         __syncwarp();
-        if (lane == 0 && s0 + ST < s1) load(s0 + ST, v_page, n % ST, 0);
+        if (leader && s0 + ST < s1) load(s0 + ST, v_page, n % ST, 0);
         for (int s = s0; s < s1; ++s, ++n) {
             const int slot = n % ST, ahead = (n + 1) % ST;
             const uint8_t* strip = ring + (2 * slot + 1) * own_half_bytes(D);
@@ -546,12 +558,12 @@ __device__ __forceinline__ void shared_own(const CUtensorMap& tmap_kv, const Sha
                 }
             }
             __syncwarp();       // (V of this strip and K of the next one have been read)
-            if (lane == 0) {
+            if (leader) {
                 if (s + ST < s1) load(s + ST, v_page, slot, 1);
                 if (s + ST + 1 < s1) load(s + ST + 1, k_page, ahead, 0);
-                v_page = k_page;
-                k_page = page_of(s + ST + 2);
             }
+            v_page = k_page;
+            k_page = page_of(s + ST + 2);
         }
         // ---- my share of the unit to scratch ----
         l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
