@@ -11,7 +11,9 @@ Reference counterparts: the ``DSKernelBase`` callables under
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -973,6 +975,7 @@ def retention_stuck() -> bool:
 # (A step makes hundreds of these calls: their checks read each attribute once, and a stream is asked for by its number. A Stream object and
 # a device guard alone cost 5 us of the 22 that a call took; it takes 9 to 12 so.)
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_I32, _F32, _LOGITS = torch.int32, torch.float32, (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _place(t: torch.Tensor, name: str) -> int:
@@ -988,19 +991,12 @@ def _elsewhere(index: int, **tensors: Optional[torch.Tensor]) -> None:
             raise ValueError(f"{name} is on {t.device}, the call is on cuda:{index}")
 
 
-class _On:
-    """The call's device as the current one, for as long as it is not anyway."""
+_HERE = contextlib.nullcontext()
 
-    def __init__(self, index: int) -> None:
-        self.guard = None if index == torch.cuda.current_device() else torch.cuda.device(index)
 
-    def __enter__(self) -> None:
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _on(index: int):
+    """The call's device as the current one, where it is not that anyway."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _rows(t: torch.Tensor, name: str) -> int:
@@ -1009,6 +1005,11 @@ def _rows(t: torch.Tensor, name: str) -> int:
     if len(st) != 2 or st[1] != 1 and shape[1] > 1:
         raise ValueError(f"{name} must be 2-D with a contiguous last dimension, got {tuple(shape)} / {st}")
     return st[0] if shape[0] > 1 else shape[1]
+
+
+@functools.lru_cache(maxsize=1024)
+def _adapter_parts(index: int, tiles: int, width: int) -> int:
+    return native.cuda_lib().hds_adapter_parts(tiles, width)       # (of the current device, which is number `index`)
 
 
 def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, scales: torch.Tensor, plan: AdapterPlan,
@@ -1046,10 +1047,10 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
     if count == 0:
         return out
     lib = native.cuda_lib()
-    with _On(index):
+    with _on(index):
         ws, n_bytes = None, 0
         if plan.tile_rows > ADAPTER_FEW:
-            n_bytes = lib.hds_adapter_parts(count, K) * T * R * 4
+            n_bytes = _adapter_parts(index, count, K) * T * R * 4
             ws = x.new_empty(n_bytes // 2)       # of this call alone: a plan may be in use on several streams, and in graphs
         rc = lib.hds_adapter_add(p_base, ld_base, x.data_ptr(), ld_x, down.data_ptr(), up.data_ptr(), scales.data_ptr(), n, R, K, N, T,
                                  plan.tiles_ptr, plan.rows_ptr, count, plan.tile_rows, p_out, ld_out, _p(ws), n_bytes, dt, _raw_stream(index))
@@ -1065,7 +1066,7 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     [rows, n_q_heads * head_dim], a sequence's new tokens being neighbouring rows in the plan's order; rows behind the last sequence are left as they
     are. ``kv_cache_layer`` [blocks, 2, n_kv_heads, block_size, head_dim] holds the new tokens' keys already; ``block_tables`` int32
     [sequences, stride]. head_dim 64 or 128, 16-bit. A group's pages are those that its first sequence's table names."""
-    index = _place(q, "q")
+    index, cache = _place(q, "q"), kv_cache_layer.shape
     ld_q, ld_out, dt, dtype = _rows(q, "q"), _rows(out, "out"), _dt(q), q.dtype
     d, H, rows = plan.head_dim, plan.n_q_heads, plan.rows
     if d not in (64, 128):
@@ -1075,11 +1076,11 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
         raise ValueError(f"q and out need {rows} rows of {H} x {d}, got {tuple(q.shape)} and {tuple(out.shape)}")
     if out.dtype != dtype or kv_cache_layer.dtype != dtype:
         raise TypeError("q, out and the cache have one type")
-    blocks = kv_cache_layer.shape[0] if kv_cache_layer.dim() == 5 else 0
-    if kv_cache_layer.shape != (blocks, 2, plan.n_kv_heads, plan.block_size, d) or not kv_cache_layer.is_contiguous():
-        raise ValueError(f"the cache must be contiguous [blocks, 2, {plan.n_kv_heads}, {plan.block_size}, {d}], got {tuple(kv_cache_layer.shape)}")
-    ld_tables = _rows(block_tables, "block_tables")
-    if block_tables.dtype != torch.int32 or block_tables.shape[0] < plan.n_seqs or block_tables.shape[1] < plan.max_blocks:
+    blocks = cache[0] if len(cache) == 5 else 0
+    if cache != (blocks, 2, plan.n_kv_heads, plan.block_size, d) or not kv_cache_layer.is_contiguous():
+        raise ValueError(f"the cache must be contiguous [blocks, 2, {plan.n_kv_heads}, {plan.block_size}, {d}], got {tuple(cache)}")
+    ld_tables, (n_tables, width) = _rows(block_tables, "block_tables"), block_tables.shape
+    if block_tables.dtype != torch.int32 or n_tables < plan.n_seqs or width < plan.max_blocks:
         raise ValueError(f"block_tables must be int32 [{plan.n_seqs}, at least {plan.max_blocks}], got {block_tables.dtype} {tuple(block_tables.shape)}")
     if not index == out.get_device() == kv_cache_layer.get_device() == block_tables.get_device():
         _elsewhere(index, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
@@ -1088,8 +1089,10 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     if rows == 0:
         return out
     lib = native.cuda_lib()
-    with _On(index):
-        n_bytes = lib.hds_paged_attention_shared_workspace_bytes(rows, H, d, plan.n_tiles, plan.p_splits, plan.n_units, plan.n_workers)
+    with _on(index):
+        n_bytes = plan.workspace_bytes
+        if not n_bytes:
+            n_bytes = plan.workspace_bytes = lib.hds_paged_attention_shared_workspace_bytes(rows, H, d, plan.n_tiles, plan.p_splits, plan.n_units, plan.n_workers)
         ws = q.new_empty(n_bytes // 2)       # of this call alone: a plan may be in use on several streams, and in graphs
         rc = lib.hds_paged_attention_shared(q.data_ptr(), ld_q, out.data_ptr(), ld_out, rows, kv_cache_layer.data_ptr(), blocks, block_tables.data_ptr(), ld_tables,
                                             plan.tiles_ptr, plan.n_tiles, plan.p_splits, plan.items_ptr, plan.workers_ptr, plan.n_workers, plan.units_ptr,
@@ -1116,44 +1119,55 @@ def _check_each(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, n: int
 
 def _check_controls(logits: torch.Tensor, out: torch.Tensor, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask,
                     mask_rows) -> Tuple[int, ...]:
-    """What :func:`logit_controls` takes, and the restatement in torch: elements between the rows of logits, out, history, bias_ids, bias and mask."""
-    ld, ld_out, shape, dtype = _rows(logits, "logits"), _rows(out, "out"), logits.shape, logits.dtype
+    """What :func:`logit_controls` takes, and the restatement in torch: elements between the rows of logits, out, history, bias_ids, bias and mask;
+    history places, biases and masks."""
+    ld, ld_out, shape, dtype, index = _rows(logits, "logits"), _rows(out, "out"), logits.shape, logits.dtype, logits.get_device()
     n, V = shape
-    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if dtype not in _LOGITS:
         raise TypeError(f"unsupported logits dtype {dtype}: bf16, fp16 or fp32")
     if out.shape != shape or out.dtype != dtype:
         raise ValueError("out must be like logits")
     if n > 65535 or V >= 1 << 30:
         raise ValueError("at most 65535 rows and a vocabulary below 2^30")
-    ld_history = ld_ids = ld_bias = ld_mask = 0
+    ld_history = ld_ids = ld_bias = ld_mask = places = n_bias = n_masks = 0
+    here, each = out.get_device() == index, (n, )
     if history is not None and history_len is not None:
-        ld_history = _check_rows(history, "history", torch.int32, n)
-        _check_each(history_len, "history_len", torch.int32, n)
-        _check_each(prompt_len, "prompt_len", torch.int32, n)
-        _check_each(repetition, "repetition", torch.float32, n)
-        _check_each(presence, "presence", torch.float32, n)
-        _check_each(frequency, "frequency", torch.float32, n)
+        ld_history, places = _check_rows(history, "history", _I32, n), history.shape[1]
+        here = here and history.get_device() == index
+        if history_len.dtype is not _I32 or history_len.shape != each or not history_len.is_contiguous():
+            _check_each(history_len, "history_len", _I32, n)
+        here = here and history_len.get_device() == index
+        if prompt_len is not None:
+            if prompt_len.dtype is not _I32 or prompt_len.shape != each or not prompt_len.is_contiguous():
+                _check_each(prompt_len, "prompt_len", _I32, n)
+            here = here and prompt_len.get_device() == index
+        for t in (repetition, presence, frequency):
+            if t is not None:
+                if t.dtype is not _F32 or t.shape != each or not t.is_contiguous():
+                    for wrong, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
+                        _check_each(wrong, name, _F32, n)
+                here = here and t.get_device() == index
     elif history is not None or history_len is not None:
         raise ValueError("a history comes with its lengths")
     elif prompt_len is not None or repetition is not None or presence is not None or frequency is not None:
         raise ValueError("penalties need a history")
     if bias is not None and bias_ids is not None:
-        ld_ids, ld_bias = _check_rows(bias_ids, "bias_ids", torch.int32, n), _check_rows(bias, "bias", torch.float32, n)
-        if bias.shape != bias_ids.shape:
+        ld_ids, ld_bias, n_bias = _check_rows(bias_ids, "bias_ids", _I32, n), _check_rows(bias, "bias", _F32, n), bias.shape[1]
+        if bias_ids.shape[1] != n_bias:
             raise ValueError("bias and bias_ids have one shape")
+        here = here and bias.get_device() == bias_ids.get_device() == index
     elif bias is not None or bias_ids is not None:
         raise ValueError("biases come with their tokens")
     if mask is not None:
-        ld_mask = _check_rows(mask, "mask", torch.int32, n if mask_rows is None else None, -(-V // 32))
-        _check_each(mask_rows, "mask_rows", torch.int32, n)
+        ld_mask, n_masks = _check_rows(mask, "mask", _I32, n if mask_rows is None else None, -(-V // 32)), mask.shape[0]
+        _check_each(mask_rows, "mask_rows", _I32, n)
+        here = here and mask.get_device() == index and (mask_rows is None or mask_rows.get_device() == index)
     elif mask_rows is not None:
         raise ValueError("mask_rows needs masks")
-    index = logits.get_device()
-    for t in (out, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask, mask_rows):
-        if t is not None and t.get_device() != index:
-            _elsewhere(index, out=out, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition, presence=presence,
-                       frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, mask_rows=mask_rows)
-    return ld, ld_out, ld_history, ld_ids, ld_bias, ld_mask
+    if not here:
+        _elsewhere(index, out=out, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition, presence=presence,
+                   frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, mask_rows=mask_rows)
+    return ld, ld_out, ld_history, ld_ids, ld_bias, ld_mask, places, n_bias, n_masks
 
 
 def logit_controls(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, history: Optional[torch.Tensor] = None,
@@ -1171,15 +1185,13 @@ def logit_controls(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, 
     index = _place(logits, "logits")
     if out is None:
         out = logits.new_empty(logits.shape)
-    ld, ld_out, ld_history, ld_ids, ld_bias, ld_mask = _check_controls(logits, out, history, history_len, prompt_len, repetition, presence, frequency,
-                                                                       bias_ids, bias, mask, mask_rows)
+    ld, ld_out, ld_history, ld_ids, ld_bias, ld_mask, places, n_bias, n_masks = _check_controls(
+        logits, out, history, history_len, prompt_len, repetition, presence, frequency, bias_ids, bias, mask, mask_rows)
     n, V = logits.shape
-    with _On(index):
-        rc = native.cuda_lib().hds_logit_controls(logits.data_ptr(), ld, out.data_ptr(), ld_out, n, V, _p(history), ld_history,
-                                                  0 if history is None else history.shape[1], _p(history_len), _p(prompt_len), _p(repetition),
-                                                  _p(presence), _p(frequency), _p(bias_ids), ld_ids, _p(bias), ld_bias,
-                                                  0 if bias is None else bias.shape[1], _p(mask), ld_mask, 0 if mask is None else mask.shape[0],
-                                                  _p(mask_rows), _dt3(logits), _raw_stream(index))
+    with _on(index):
+        rc = native.cuda_lib().hds_logit_controls(logits.data_ptr(), ld, out.data_ptr(), ld_out, n, V, _p(history), ld_history, places, _p(history_len),
+                                                  _p(prompt_len), _p(repetition), _p(presence), _p(frequency), _p(bias_ids), ld_ids, _p(bias), ld_bias,
+                                                  n_bias, _p(mask), ld_mask, n_masks, _p(mask_rows), _dt3(logits), _raw_stream(index))
     if rc:
         native.check(rc, "hds_logit_controls")
     _count(1 if n and V else 0)

@@ -127,6 +127,8 @@ class SharedPrefixPlan:
         items[:, 4], items[:, 5], items[:, 6] = prefix, unit0[:-1], row_tiles
         self.items, self.workers, self.units = items, workers.astype(np.int32), units.astype(np.int32)
         self.device = None if device is None else torch.device(device)
+        #: bytes of a call's scratch (0: the library has not been asked yet)
+        self.workspace_bytes = 0
         #: device number (-1: not on a GPU) and device pointers
         self.index = -1
         if self.device is not None and self.device.type == "cuda":
