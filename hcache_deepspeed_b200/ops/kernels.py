@@ -1,7 +1,7 @@
 """torch-facing wrappers over the sm_100a kernel library (``include/hds_b200.h``).
 
 Every function takes CUDA tensors, launches on the current stream and returns immediately; there
-is no hidden allocation unless an ``out=`` argument is omitted. These wrappers are the ONLY way the
+is no hidden allocation unless an ``out=`` argument is omitted or the function's docstring says so. These wrappers are the ONLY way the
 framework runs compute on the device — there is no eager-PyTorch fallback behind them (the fp32
 PyTorch restatements used as test oracles live in :mod:`hcache_deepspeed_b200.ops.reference`).
 
@@ -14,6 +14,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import math
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -1016,7 +1017,8 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[t] = base[t] + scales[i] * (x[t] @ down[i].T) @ up[i].T`` with row t's own adapter ``i`` (``plan``), ``out[t] = base[t]`` for a row
     without one. ``base`` [T, N] (the shared projection's output), ``x`` [T, K], ``down`` [adapters, R, K], ``up`` [adapters, N, R], 16-bit;
-    ``scales`` fp32 [adapters]. K, N and R are multiples of 8, R at most 256. ``out`` may be ``base``."""
+    ``scales`` fp32 [adapters]. K, N and R are multiples of 8, R at most 256. ``out`` may be ``base`` or ``x``. With more than 16 rows of an
+    adapter the call allocates scratch."""
     index = _place(x, "x")
     ld_x, ld_base, dt, dtype = _rows(x, "x"), _rows(base, "base"), _dt(x), x.dtype
     (T, K), (rows, N) = x.shape, base.shape
@@ -1065,7 +1067,8 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     """Causal attention of a batch whose sequences share prefixes (``plan``), each prefix read once for its group. ``q`` and ``out``
     [rows, n_q_heads * head_dim], a sequence's new tokens being neighbouring rows in the plan's order; rows behind the last sequence are left as they
     are. ``kv_cache_layer`` [blocks, 2, n_kv_heads, block_size, head_dim] holds the new tokens' keys already; ``block_tables`` int32
-    [sequences, stride]. head_dim 64 or 128, 16-bit. A group's pages are those that its first sequence's table names."""
+    [sequences, stride]. head_dim 64 or 128, 16-bit. A group's pages are those that its first sequence's table names. Finite ``scale`` of 0 or more.
+    The call allocates its scratch."""
     index, cache = _place(q, "q"), kv_cache_layer.shape
     ld_q, ld_out, dt, dtype = _rows(q, "q"), _rows(out, "out"), _dt(q), q.dtype
     d, H, rows = plan.head_dim, plan.n_q_heads, plan.rows
@@ -1086,6 +1089,8 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
         _elsewhere(index, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
     if plan.index != index:
         raise ValueError(f"the plan is on {plan.device}, the call is on cuda:{index}")
+    if not 0.0 <= scale < math.inf:
+        raise ValueError(f"scale must be finite and not negative, got {scale}")
     if rows == 0:
         return out
     lib = native.cuda_lib()

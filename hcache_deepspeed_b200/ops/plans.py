@@ -55,8 +55,9 @@ class AdapterPlan:
         #: device number (-1: not on a GPU) and device pointers
         self.index, self.tiles_ptr, self.rows_ptr = -1, 0, 0
         if self.device is not None and self.device.type == "cuda":
-            places = np.asarray([[min(start + r, start + n - 1) for r in range(ADAPTER_ROWS)] for _, start, n, _ in tiles], dtype=np.int64).reshape(-1, ADAPTER_ROWS)
-            self._dev = torch.from_numpy(np.concatenate([np.asarray(tiles, dtype=np.int32).reshape(-1), order[places].reshape(-1)])).to(self.device)
+            flat = np.asarray(tiles, dtype=np.int32).reshape(-1, 4)
+            places = flat[:, 1:2] + np.minimum(np.arange(ADAPTER_ROWS, dtype=np.int32), flat[:, 2:3] - 1)      # (the last row again where a tile ends)
+            self._dev = torch.from_numpy(np.concatenate([flat.reshape(-1), order[places].reshape(-1)])).to(self.device)
             self.index, self.tiles_ptr = self._dev.get_device(), self._dev.data_ptr()
             self.rows_ptr = self.tiles_ptr + 16 * len(tiles)
 

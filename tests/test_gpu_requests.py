@@ -82,6 +82,24 @@ def test_adapters_of_rows_apart_in_memory(dtype):
     assert (wide_out[:, :8] == 9).all() and (wide_out[:, 144:] == 9).all()
 
 
+@pytest.mark.parametrize("rows", [6, 40])       # one kernel, and two
+def test_adapters_of_rows_far_apart_and_in_place_of_x(rows):
+    ids, ld = [0] * (rows - 2) + [1, -1], 1 << 27
+    base, x, down, up, scales = adapters_inputs(rows, 2, 520, 520, 24, torch.bfloat16)
+    plan = K().AdapterPlan(ids, 2, device="cuda")
+    want, bound = adapters_exact(base, x, down, up, scales, ids)
+    wide = torch.empty(rows, ld, dtype=torch.bfloat16, device="cuda")
+    far, x_far = wide[:, ld - 520:], wide[:, :520]
+    far.copy_(base)
+    x_far.copy_(x)
+    K().adapter_add(far, x_far, down, up, scales, plan, out=far)
+    check(far, want, bound)
+    far.copy_(base)
+    K().adapter_add(far, x_far, down, up, scales, plan, out=x_far)
+    check(x_far, want, bound)
+    assert torch.equal(far, base)
+
+
 def test_adapters_keep_large_and_small_sums():
     """fp16: h of 10^5 has no place in 16 bits, h of 10^-6 few bits."""
     torch.manual_seed(2)
@@ -275,6 +293,31 @@ def test_attention_takes_rows_apart_in_memory(dtype):
     assert torch.equal(out[:, 16:272], dense) and (out[:, :16] == 5).all() and (out[:, 272:] == 5).all()
 
 
+def test_attention_in_a_cache_of_more_than_2_to_32_values():
+    torch.manual_seed(9)
+    new, keys, groups, kvh, d, bs = [1, 2], [256 + 30, 256 + 140], [(0, 2, 256)], 8, 128, 128
+    small, tables = pages(keys, groups, kvh, d, bs, torch.bfloat16)
+    n, first = small.shape[0], 17000
+    cache = torch.empty(first + n, 2, kvh, bs, d, dtype=torch.bfloat16, device="cuda")
+    assert cache.numel() > 1 << 32
+    cache[first:] = small
+    plan = K().SharedPrefixPlan(new, keys, groups, 16, kvh, d, bs, device="cuda")
+    q = rand(3, 16 * d, std=2.0)
+    out = K().paged_attention_shared(q, torch.empty_like(q), cache, tables + first, plan, d**-0.5)
+    assert torch.equal(out, K().paged_attention_shared(q, torch.empty_like(q), small, tables, plan, d**-0.5))
+    check(out, *attention_exact(q, small, tables, new, keys, [256, 256], 16, d**-0.5))
+
+
+def test_attention_may_write_over_its_queries():
+    torch.manual_seed(10)
+    new, keys, groups = [1, 2], [150, 170], [(0, 2, 128)]
+    cache, tables = pages(keys, groups, 2, 64, 32, torch.float16)
+    plan = K().SharedPrefixPlan(new, keys, groups, 8, 2, 64, 32, device="cuda")
+    q = rand(3, 512, dtype=torch.float16)
+    want = K().paged_attention_shared(q, torch.empty_like(q), cache, tables, plan, 0.125)
+    assert torch.equal(K().paged_attention_shared(q, q, cache, tables, plan, 0.125), want)
+
+
 def test_attention_refuses():
     k = K()
     plan = k.SharedPrefixPlan([1, 1], [40, 40], [(0, 2, 32)], 4, 2, 64, 16, device="cuda")
@@ -286,6 +329,7 @@ def test_attention_refuses():
                     (dict(block_tables=good["block_tables"][:1]), ValueError), (dict(block_tables=good["block_tables"][:, :2]), ValueError),
                     (dict(block_tables=good["block_tables"].long()), ValueError), (dict(block_tables=good["block_tables"].cpu()), ValueError),
                     (dict(plan=k.SharedPrefixPlan([1, 1], [40, 40], [], 4, 2, 64, 16)), ValueError),
+                    (dict(scale=-0.125), ValueError), (dict(scale=math.inf), ValueError), (dict(scale=math.nan), ValueError),
                     (dict(plan=k.SharedPrefixPlan([1, 1], [40, 40], [], 4, 2, 96, 16, device="cuda"), q=rand(2, 384), out=rand(2, 384)), ValueError)):
         with pytest.raises(err):
             k.paged_attention_shared(**{**good, **kw})
@@ -408,6 +452,16 @@ def test_controls_of_rows_on_any_address(dtype):
         K().logit_controls(wide[:, shift_in:shift_in + 301], out[:, shift_out:shift_out + 301], **c)
         controls_check(out[:, shift_out:shift_out + 301], want, bound)
         assert (out[:, :shift_out] == 3).all() and (out[:, shift_out + 301:] == 3).all()
+
+
+def test_controls_of_rows_far_apart():
+    V, ld = 5000, 1 << 28
+    logits, c = controls_inputs(10, V, torch.float16, 900, 7, 1)
+    want, bound = controls_exact(logits, **c)
+    wide = torch.empty(10, ld, dtype=torch.float16, device="cuda")
+    wide[:, :V] = logits
+    K().logit_controls(wide[:, :V], wide[:, ld - V:], **c)
+    controls_check(wide[:, ld - V:], want, bound)
 
 
 def test_controls_pass_infinities_and_nan_on():

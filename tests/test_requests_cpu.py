@@ -134,6 +134,14 @@ def test_own_keys_are_dealt_out_whole(new, keys, groups, H, kvh):
     assert len({u + w for u, w in shares}) == len(shares) and max((u + w for u, w in shares), default=-1) < plan.n_units + plan.n_workers
 
 
+@pytest.mark.parametrize("scale", [-1.0, float("inf"), float("nan")])
+def test_attention_refuses_scales_that_are_none(scale):
+    plan = plans.SharedPrefixPlan([1, 1], [40, 40], [(0, 2, 32)], 4, 2, 64, 16)
+    q = torch.zeros(2, 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="scale"):
+        CpuOps().attention_shared(q, torch.empty_like(q), torch.zeros(9, 2, 2, 16, 64, dtype=torch.bfloat16), torch.zeros(2, 3, dtype=torch.int32), plan, scale)
+
+
 def test_attention_of_a_group_on_the_host_is_that_of_its_sequences():
     torch.manual_seed(1)
     plan = plans.SharedPrefixPlan([1, 3, 0, 2], [40, 45, 33, 5], [(0, 3, 32)], 6, 2, 32, 16)
