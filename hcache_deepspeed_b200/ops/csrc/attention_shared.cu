@@ -8,9 +8,12 @@
 //    same keys; with fewer they share the rows and take the key tiles in turn, as two more parts of the prefix.
 //      warp 0    : TMA producer - Q (3-D boxes: tokens x heads x 64 dims), then K and V tiles page by page in the order of their use, through one
 //                  ring; what is behind the prefix in its last tile comes from behind the cache, that is, as zeros
-//      warp 1    : TMEM allocator, tcgen05.mma issuer: O += P V, then S = Q K^T of the stream's next tile (V MN-major, as its pages have it)
+//      warp 1    : TMEM allocator, tcgen05.mma issuer, for half a tile at a time: O += P V, then S = Q K^T of the same half of the stream's next tile
+//                  (V MN-major, as its pages have it)
 //      warps 2-9 : softmax, four warps per stream, one thread per row; P goes back to TMEM as 16-bit pairs, over the scores it came from. O stays in
-//                  TMEM and is rescaled only when a row's maximum grows by more than 2^8
+//                  TMEM and is rescaled only when a row's maximum grows by more than 2^8. One half is weighed while the other half's products run:
+//                  with products of whole tiles a stream waits for them between two tiles (56.0 us here, 58.4 so at the 65536 keys below; 38.3 and
+//                  38.0 at the 8192, where the issue of twice as many products weighs more)
 //    No causal edge: every row comes behind the whole prefix. (m, l, O) in fp32 go to scratch, one part per split and key stream.
 // 2. Own keys. The warps of a CTA are twelve workers: each takes strips of 16 keys through a ring of its own (TMA, see attention_group.cu, whose
 //    arithmetic this is: up to 8 query rows of a sequence and KV head, mma.sync, the weights' rounding kept in the MMA's other 8 rows). All
@@ -19,17 +22,19 @@
 //    heads of a short sequence came 25 us behind the others). (m, l, O) of a sequence's share in a piece goes to scratch.
 //    These CTAs are of the prefix' launch and begin with it, on so many SMs that both should end together: own keys wait for memory where
 //    the prefix waits for its softmax. (One after the other, 4096 shared keys and 32 sequences of 32 heads with 150 keys each took 41.4 us, 64 sequences
-//    of 64 heads behind 8192 keys 48.0; together 35.7 and 42.3.)
+//    of 64 heads behind 8192 keys 48.0; together 35.7 and 42.3. Both parts have become faster since.)
 // 3. The end: the parts of every row, from prefix and own keys, join in a kernel of their own. The scratch has no counters and no state between calls.
 //
 // Measured (bf16, bytes that any form has to move, time, bytes per second; a copy runs at 6.55 TB/s):
-//   32 sequences, 32 heads of 128 dims and as many KV heads, prefix 4096, 1 to 300 own keys: 147 MB, 35.7 us, 4.1 TB/s
-//   64 sequences, 64 heads on 8, prefix 8192, 1 to 600 own keys:                             118 MB, 42.3 us, 2.8 TB/s: the prefix' softmax, see below
-//   77 sequences, 32 heads on 8, up to 3 new tokens, prefixes 2048 and 1024, 1 to 500 own:    93 MB, 34.8 us, 2.7 TB/s: own keys once per 8 rows, 2 and 3 tokens have 12
-//   9 sequences, 64 heads on 8, prefix 65536, 1 to 1500 own keys:                             294 MB, 61.6 us, 4.8 TB/s
-//   4 sequences, 12 heads of 64 dims (fp16), prefix 512, 1 to 90 own keys:                    9.5 us: two kernels' beginnings, 5 us + 3 us
-// A key tile takes a CTA 1.3 us, or 2.9 us under two row tiles, where products and exponentials alone are 0.55 and 1.07 us: the way of one stream's
-// scores from TMEM through maximum, weights and back is 2.5 us long, and TMEM has room for two streams.
+//   32 sequences, 32 heads of 128 dims and as many KV heads, prefix 4096, 1 to 300 own keys:  147 MB, 32.3 us, 4.6 TB/s
+//   64 sequences, 64 heads on 8, prefix 8192, 1 to 600 own keys:                              118 MB, 38.3 us, 3.1 TB/s
+//   77 sequences, 32 heads on 8, 1 to 3 new tokens, prefixes 2048 and 1024, 1 to 500 own keys: 93 MB, 30.8 us, 3.0 TB/s
+//   9 sequences, 64 heads on 8, prefix 65536, 1 to 1500 own keys:                             294 MB, 56.0 us, 5.3 TB/s
+//   4 sequences, 12 heads of 64 dims (fp16), prefix 512, 1 to 90 own keys: 8.7 us, two kernels' beginnings and ends (5 + 3)
+// The join and the beginnings are 6 to 8 us of each. Under two row tiles (the second and third line) a key tile takes 2.0 us of a CTA, of which its
+// products are 1.1 and its exponentials 1.1: registers and TMEM have room for two streams. Own keys come at 6 TB/s where sequences are long (1200 keys);
+// with 150 a worker begins a sequence and head every nine strips. Tokens of which a sequence has two or three have two units of 8 rows, which read the keys
+// twice (once from L2).
 //
 // P is rounded to 16 bits in the first part: each weight by half a step of its own (2^-9 in bf16, 2^-12 in fp16, where the weights are held 2^7
 // larger so that small ones keep their bits), which averages out over the keys; sums are of the unrounded weights.

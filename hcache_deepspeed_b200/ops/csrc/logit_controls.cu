@@ -16,6 +16,12 @@
 // A row may begin on any element: chunks are cut at 16-byte boundaries of the logits, so that all but a row's two ends are moved 16 bytes at a
 // time.
 //
+// Measured (bytes that any form has to move, time, bytes per second; a copy runs at 6.55 TB/s):
+//   1 row of 50272 (fp16), history of 700: 2.5 us, the chain of one CTA: ids, table, list
+//   64 rows of 32000 (bf16), histories of up to 4096, 300 biases, masks: 9 MB, 13.0 us: a CTA counts 4096 ids for 8192 logits
+//   256 rows of 131071 (fp32), histories of up to 8192, 64 biases, masks: 275 MB, 76.5 us, 3.6 TB/s: the same, in seven waves of CTAs, of whose 10 us
+//   the logits are on the way for 3; chunks of 16384 and 32768 take 74.9 and 70.0 us, but 17.6 and 28.1 at the 64 rows
+//
 // No counterpart in the reference, which leaves the choice of tokens to its caller.
 #include "hds_ptx.cuh"
 #include "hds_host.cuh"
