@@ -1,6 +1,7 @@
 """Token sampling over last-token logits (the reference leaves this to HF ``generate`` / DeepSpeed-MII)."""
 from __future__ import annotations
 
+import math
 from typing import Dict, List, Optional, Sequence, Union
 
 import torch
@@ -27,8 +28,10 @@ class LogitControls:
         told = [torch.as_tensor(p).reshape(-1).to(torch.int32).cpu() for p in prompts]
         each = lambda v, name: self._each(v, n, name)  # noqa: E731
         rep, pres, freq = each(repetition_penalty, "repetition_penalty"), each(presence_penalty, "presence_penalty"), each(frequency_penalty, "frequency_penalty")
-        if any(not r > 0 for r in rep):
-            raise ValueError("repetition_penalty must be positive")
+        if any(not 0 < r < math.inf for r in rep):
+            raise ValueError("repetition_penalty must be positive and finite")
+        if not all(map(math.isfinite, pres + freq)):
+            raise ValueError("presence_penalty and frequency_penalty must be finite")
         self._c = {}
         self._room = 0
         if any(r != 1 for r in rep) or any(pres) or any(freq):
@@ -47,6 +50,8 @@ class LogitControls:
             k = max(map(len, lists), default=0)
             if any(not 0 <= t < vocab for b in lists for t in b):
                 raise ValueError("logit_bias names a token outside the vocabulary")
+            if any(not v < math.inf for b in lists for v in b.values()):
+                raise ValueError("logit_bias must be finite, or -inf")
             self._c["bias_ids"] = torch.tensor([list(b) + [-1] * (k - len(b)) for b in lists], dtype=torch.int32).reshape(n, k)
             self._c["bias"] = torch.tensor([list(b.values()) + [0.0] * (k - len(b)) for b in lists], dtype=torch.float32).reshape(n, k)
         self._c = {name: t.to(self.device) for name, t in self._c.items()}
@@ -101,12 +106,21 @@ class LogitControls:
         self.n = len(places)
 
 
+def _drawable(logits: torch.Tensor) -> torch.Tensor:
+    """Logits whose softmax is a distribution whatever the controls left of them (drawing from anything else ends a GPU's context): an infinite one
+    is a very large one, and a row without any token has token 0, as the arg-max has it."""
+    x = torch.nan_to_num(logits.float(), nan=-math.inf, posinf=1e30, neginf=-math.inf)
+    x[:, 0] = torch.where(x.amax(-1) == -math.inf, 0.0, x[:, 0])
+    return x
+
+
 def sample_next(logits: torch.Tensor, do_sample: bool = False, temperature: float = 1.0, top_k: int = 0,
                 top_p: float = 1.0, controls: Optional[LogitControls] = None) -> torch.Tensor:
     """``logits [n, vocab]`` -> int32 ``[n]``. Greedy decoding runs the library's arg-max kernel on a GPU. ``controls`` are laid on the logits first,
     and told the tokens."""
     if controls is not None:
-        tokens = sample_next(controls.apply(logits), do_sample, temperature, top_k, top_p)
+        left = controls.apply(logits)
+        tokens = sample_next(_drawable(left) if do_sample and temperature != 0.0 else left, do_sample, temperature, top_k, top_p)
         controls.append(tokens)
         return tokens
     if not do_sample or temperature == 0.0:

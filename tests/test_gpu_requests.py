@@ -577,3 +577,8 @@ def test_tokens_under_controls_on_the_gpu():
         if step == 3:
             a.keep([0, 2])
             b.keep([0, 2])
+
+
+def test_drawing_where_controls_leave_no_token_on_the_gpu():
+    from test_requests_cpu import draws_with_no_token_left
+    draws_with_no_token_left("cuda")
