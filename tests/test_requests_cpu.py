@@ -216,21 +216,17 @@ def test_controls_without_any_leave_logits_alone():
     assert sample_next(logits, controls=controls).tolist() == logits.argmax(-1).tolist()
 
 
-def draws_with_no_token_left(device):
+def test_drawing_where_controls_leave_no_token():
     """Rows: nothing allowed, nothing left by the bias, one token left, an infinite logit."""
     allowed = torch.ones(4, 5, dtype=torch.bool)
     allowed[0] = False
     allowed[1, 2:] = False
     allowed[2] = torch.tensor([False, False, False, True, False])
-    controls = LogitControls([[1]] * 4, 5, 6, device, 1.5, logit_bias=[None, {0: -math.inf, 1: -math.inf}, None, None], allowed=allowed)
-    logits = torch.zeros(4, 5, device=device)
+    controls = LogitControls([[1]] * 4, 5, 6, "cpu", 1.5, logit_bias=[None, {0: -math.inf, 1: -math.inf}, None, None], allowed=allowed)
+    logits = torch.zeros(4, 5)
     logits[3, 4] = math.inf
     for kw in ({}, dict(top_k=2), dict(top_p=0.5), dict(temperature=1e-9), dict(temperature=3.0, top_k=1, top_p=0.9)):
         assert sample_next(logits, do_sample=True, controls=controls, **kw).tolist() == [0, 0, 3, 4]
-
-
-def test_drawing_where_controls_leave_no_token():
-    draws_with_no_token_left("cpu")
 
 
 def test_controls_refuse():
