@@ -20,7 +20,7 @@
 //   1 row of 50272 (fp16), history of 700: 2.5 us, the chain of one CTA: ids, table, list
 //   64 rows of 32000 (bf16), histories of up to 4096, 300 biases, masks: 9 MB, 13.0 us: a CTA counts 4096 ids for 8192 logits
 //   256 rows of 131071 (fp32), histories of up to 8192, 64 biases, masks: 275 MB, 76.5 us, 3.6 TB/s: the same, in seven waves of CTAs, of whose 10 us
-//   the logits are on the way for 3; chunks of 16384 and 32768 take 74.9 and 70.0 us, but 17.6 and 28.1 at the 64 rows. Histories dealt out by chunk
+//   the logits are on the way for 3, and 73% of the issue slots; chunks of 16384 and 32768 take 74.9 and 70.0 us, but 17.6 and 28.1 at the 64 rows. Histories dealt out by chunk
 //   in a kernel of its own beside the stream: 74.3 us, for two launches; CTAs that ask for their next chunk before they count this one's: 105 us, as
 //   only two of them have registers
 //
