@@ -1050,12 +1050,14 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
         return out
     lib = native.cuda_lib()
     with _on(index):
+        stream = _raw_stream(index)
+        plan.used_on(stream)
         ws, n_bytes = None, 0
         if plan.tile_rows > ADAPTER_FEW:
             n_bytes = _adapter_parts(index, count, K) * T * R * 4
             ws = x.new_empty(n_bytes // 2)       # of this call alone: a plan may be in use on several streams, and in graphs
         rc = lib.hds_adapter_add(p_base, ld_base, x.data_ptr(), ld_x, down.data_ptr(), up.data_ptr(), scales.data_ptr(), n, R, K, N, T,
-                                 plan.tiles_ptr, plan.rows_ptr, count, plan.tile_rows, p_out, ld_out, _p(ws), n_bytes, dt, _raw_stream(index))
+                                 plan.tiles_ptr, plan.rows_ptr, count, plan.tile_rows, p_out, ld_out, _p(ws), n_bytes, dt, stream)
     if rc:
         native.check(rc, "hds_adapter_add")
     _count(1 if ws is None else 2)
@@ -1095,6 +1097,8 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
         return out
     lib = native.cuda_lib()
     with _on(index):
+        stream = _raw_stream(index)
+        plan.used_on(stream)
         n_bytes = plan.workspace_bytes
         if not n_bytes:
             n_bytes = plan.workspace_bytes = lib.hds_paged_attention_shared_workspace_bytes(rows, H, d, plan.n_tiles, plan.p_splits, plan.n_units, plan.n_workers)
@@ -1102,7 +1106,7 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
         rc = lib.hds_paged_attention_shared(q.data_ptr(), ld_q, out.data_ptr(), ld_out, rows, kv_cache_layer.data_ptr(), blocks, block_tables.data_ptr(), ld_tables,
                                             plan.tiles_ptr, plan.n_tiles, plan.p_splits, plan.items_ptr, plan.workers_ptr, plan.n_workers, plan.units_ptr,
                                             plan.n_units, plan.rows_ptr, H, plan.n_kv_heads, d, plan.block_size, scale, ws.data_ptr(), n_bytes, dt,
-                                            _raw_stream(index))
+                                            stream)
     if rc:
         native.check(rc, "hds_paged_attention_shared")
     _count(2)

@@ -1,7 +1,8 @@
 """What the host works out once per batch for the kernels that share work among its requests; every layer's calls take the same plan.
 
 A plan belongs to one batch. Its arrays are on the device when the constructor returns, and no call changes them: calls on any stream, and
-captured graphs, may share one."""
+captured graphs, may share one. It may be dropped while calls are still on their way, on whatever stream; only a captured graph does not keep it
+alive: as long as that is replayed, its plans have to be kept, as its other inputs."""
 from __future__ import annotations
 
 from typing import Sequence, Tuple
@@ -28,7 +29,28 @@ def _host_ints(values, name: str) -> np.ndarray:
     return a.astype(np.int64)
 
 
-class AdapterPlan:
+class _Plan:
+    """Where a plan's arrays are."""
+
+    #: device number (-1: not on a GPU), its memory, the stream that this belongs to, and the others that have calls with it
+    index, _dev, _stream, _others = -1, None, 0, frozenset()
+
+    def _place(self, flat: np.ndarray, device: torch.device) -> int:
+        """The int32 values ``flat`` to the GPU ``device``; where they are."""
+        self._dev = torch.from_numpy(flat).to(device)
+        self.index = self._dev.get_device()
+        self._stream = torch._C._cuda_getCurrentRawStream(self.index)
+        return self._dev.data_ptr()
+
+    def used_on(self, stream: int) -> None:
+        """A call on the current stream of the plan's device, which has that number, reads the arrays: their memory is not given to anybody else
+        ahead of its end."""
+        if stream != self._stream and stream not in self._others:
+            self._dev.record_stream(torch.cuda.current_stream(self.index))
+            self._others = self._others | {stream}
+
+
+class AdapterPlan(_Plan):
     """Which rows go through which adapter. ``ids[t]``: the adapter of row t, negative for none. ``device``: where the calls run (host
     memory: only the restatement in torch does)."""
 
@@ -52,17 +74,16 @@ class AdapterPlan:
         self.n_tiles_and_bare = len(tiles)
         self.tiles = tiles
         self.device = None if device is None else torch.device(device)
-        #: device number (-1: not on a GPU) and device pointers
-        self.index, self.tiles_ptr, self.rows_ptr = -1, 0, 0
+        #: device pointers
+        self.tiles_ptr, self.rows_ptr = 0, 0
         if self.device is not None and self.device.type == "cuda":
             flat = np.asarray(tiles, dtype=np.int32).reshape(-1, 4)
             places = flat[:, 1:2] + np.minimum(np.arange(ADAPTER_ROWS, dtype=np.int32), flat[:, 2:3] - 1)      # (the last row again where a tile ends)
-            self._dev = torch.from_numpy(np.concatenate([flat.reshape(-1), order[places].reshape(-1)])).to(self.device)
-            self.index, self.tiles_ptr = self._dev.get_device(), self._dev.data_ptr()
+            self.tiles_ptr = self._place(np.concatenate([flat.reshape(-1), order[places].reshape(-1)]), self.device)
             self.rows_ptr = self.tiles_ptr + 16 * len(tiles)
 
 
-class SharedPrefixPlan:
+class SharedPrefixPlan(_Plan):
     """A batch whose sequences share prefixes. ``new_tokens[i]`` query rows of sequence i (in this order in ``q``), behind ``keys[i]`` -
     ``new_tokens[i]`` earlier tokens; ``groups``: (first sequence, sequences, prefix) - the block tables of these neighbouring sequences
     begin with the same pages, for ``prefix`` tokens (a multiple of the block size, and none of the new ones). Sequences in no group share nothing."""
@@ -130,15 +151,11 @@ class SharedPrefixPlan:
         self.device = None if device is None else torch.device(device)
         #: bytes of a call's scratch (0: the library has not been asked yet)
         self.workspace_bytes = 0
-        #: device number (-1: not on a GPU) and device pointers
-        self.index = -1
         if self.device is not None and self.device.type == "cuda":
             row_items = np.repeat(np.arange(new.size), new).astype(np.int32)
             parts = [np.asarray(tiles, dtype=np.int32), items, self.workers, self.units, row_items]       # all but the last start on 16-byte boundaries
             flat = [np.concatenate([p.reshape(-1), np.zeros(-p.size % 4, dtype=np.int32)]) for p in parts]
-            self._dev = torch.from_numpy(np.concatenate(flat)).to(self.device)
-            self.index = self._dev.get_device()
-            at = self._dev.data_ptr() + 4 * np.cumsum([0] + [f.size for f in flat])
+            at = self._place(np.concatenate(flat), self.device) + 4 * np.cumsum([0] + [f.size for f in flat])
             self.tiles_ptr, self.items_ptr, self.workers_ptr, self.units_ptr, self.rows_ptr = at[:5].tolist()
 
 

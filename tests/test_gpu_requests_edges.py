@@ -1,0 +1,39 @@
+"""Batches of many requests at their edges, on the GPU. Oracles and tolerances are those of test_gpu_requests.py."""
+import pytest
+import torch
+
+from tests.test_gpu_requests import K, adapters_exact, adapters_inputs, attention_exact, check, pages, rand
+
+pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
+
+
+@pytest.mark.parametrize("which", ["adapters", "shared"])
+def test_a_plan_that_is_dropped_keeps_its_memory_until_its_calls_end(which):
+    """Made on one stream, used on another that is busy, and dropped: what the first stream allocates next lies elsewhere."""
+    torch.manual_seed(0)
+    busy = torch.cuda.Stream()
+    if which == "adapters":
+        ids = [0, 1, -1, 1]
+        inputs = adapters_inputs(4, 2, 64, 64, 8, torch.bfloat16)
+        plan = K().AdapterPlan(ids, 2, device="cuda")
+        call = lambda plan: K().adapter_add(*inputs, plan)  # noqa: E731
+        want, bound = adapters_exact(*inputs, ids)
+    else:
+        new, keys, groups = [1, 2], [70, 75], [(0, 2, 64)]
+        cache, tables = pages(keys, groups, 2, 64, 32, torch.bfloat16)
+        q = rand(3, 256)
+        plan = K().SharedPrefixPlan(new, keys, groups, 4, 2, 64, 32, device="cuda")
+        call = lambda plan: K().paged_attention_shared(q, torch.empty_like(q), cache, tables, plan, 0.125)  # noqa: E731
+        want, bound = attention_exact(q, cache, tables, new, keys, [64, 64], 4, 0.125)
+    call(plan)
+    torch.cuda.synchronize()
+    at, n = plan._dev.data_ptr(), plan._dev.numel()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(200_000_000)
+        out = call(plan)
+    del plan
+    later = [torch.empty(n, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not busy.query(), "the stream was to be busy still"
+    assert at not in [t.data_ptr() for t in later]
+    torch.cuda.synchronize()
+    check(out, want, bound)

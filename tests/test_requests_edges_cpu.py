@@ -1,0 +1,82 @@
+"""Batches of many requests at their edges, on the host: what plans keep alive, what the wrappers hand to the library and what they refuse."""
+import pytest
+import torch
+
+from hcache_deepspeed_b200.ops import kernels, native, plans
+
+
+# ---- the wrappers against a library that only notes its calls ------------------------------------------------------------
+class OnGpu(torch.Tensor):
+    """A tensor in host memory that says it is on GPU 0."""
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return 0
+
+
+def gpu(t):
+    return torch.Tensor._make_subclass(OnGpu, t)
+
+
+class Noted:
+    """Every entry point notes its arguments and is content."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        if name.startswith("hds_"):
+            return lambda *args: self.calls.append((name, args)) or 0
+        raise AttributeError(name)
+
+
+class Memory:
+    """Device memory of a plan that notes which streams it was recorded for."""
+
+    def __init__(self):
+        self.recorded = []
+
+    def record_stream(self, stream):
+        self.recorded.append(stream)
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    import contextlib
+    noted = Noted()
+    monkeypatch.setattr(native, "cuda_lib", lambda: noted)
+    monkeypatch.setattr(kernels, "_on", lambda index: contextlib.nullcontext())
+    noted.stream = 0
+    monkeypatch.setattr(kernels, "_raw_stream", lambda index: noted.stream)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: noted.stream)
+    return noted
+
+
+def placed(plan):
+    """The plan as if its arrays were on GPU 0, made on stream 0."""
+    plan.index, plan._dev = 0, Memory()
+    for name in ("tiles_ptr", "items_ptr", "workers_ptr", "units_ptr", "rows_ptr"):
+        setattr(plan, name, 0)
+    return plan
+
+
+def adapters_call(T=3, n=2, K=16, N=8, R=8):
+    bf = lambda *s: gpu(torch.zeros(*s, dtype=torch.bfloat16))  # noqa: E731
+    return dict(base=bf(T, N), x=bf(T, K), down=bf(n, R, K), up=bf(n, N, R), scales=gpu(torch.zeros(n)), plan=placed(kernels.AdapterPlan([i % n for i in range(T)], n)))
+
+
+def shared_call(n=2):
+    bf = lambda *s: gpu(torch.zeros(*s, dtype=torch.bfloat16))  # noqa: E731
+    return dict(q=bf(n, 128), out=bf(n, 128), kv_cache_layer=bf(9, 2, 2, 16, 64), block_tables=gpu(torch.zeros(n, 3, dtype=torch.int32)), scale=0.125,
+                plan=placed(plans.SharedPrefixPlan([1] * n, [40] * n, [(0, n, 32)], 2, 2, 64, 16)))
+
+
+@pytest.mark.parametrize("call,args", [(kernels.adapter_add, adapters_call), (kernels.paged_attention_shared, shared_call)])
+def test_a_plan_outlives_its_calls_on_other_streams(lib, call, args):
+    """Its memory belongs to the stream that it was made on: for any other one that reads it, it has to be recorded, or a plan that is dropped gives its
+    memory away under a running kernel."""
+    kw = args()
+    for lib.stream in (0, 7, 7, 0, 9, 7):
+        call(**kw)
+    assert len([c for c in lib.calls if c[0] in ("hds_adapter_add", "hds_paged_attention_shared")]) == 6
+    assert kw["plan"]._dev.recorded == [7, 9]
