@@ -790,7 +790,10 @@ extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out
     a.num_rows_kv = static_cast<int>(kv_rows);
     a.tile_tokens = 128 / G;
     a.p_splits = p_splits;
-    a.scale_log2 = scale * 1.4426950408889634f;
+    // Keys that are masked enter as scores of -inf, which are to stay that whatever the scale: a scale of 0 counts as the smallest number above it,
+    // which moves no exponent by 2^-20 (scores are below 2^128).
+    const float scale_log2 = scale * 1.4426950408889634f;
+    a.scale_log2 = scale_log2 > 0.0f ? scale_log2 : 1.401298464e-45f;
     // the outputs first: they want 32-byte boundaries
     const int64_t parts = n_tiles > 0 ? static_cast<int64_t>(2 * p_splits) * rows * n_q_heads : 0;
     const int64_t shares = (static_cast<int64_t>(n_units) + n_workers) * kOwnRows;

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from tests.test_gpu_requests import K, adapters_exact, adapters_inputs, attention_exact, check, pages, rand
+from tests.test_gpu_requests import HALF, K, adapters_exact, adapters_inputs, attention_exact, check, pages, rand
 
 pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
 
@@ -37,3 +37,18 @@ def test_a_plan_that_is_dropped_keeps_its_memory_until_its_calls_end(which):
     assert at not in [t.data_ptr() for t in later]
     torch.cuda.synchronize()
     check(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("prefix,bs", [(16, 16), (144, 16), (192, 64), (1088, 64)])
+@pytest.mark.parametrize("scale", [0.0, 1e-46, 1e-40])      # (1e-46 is 0 in 32 bits)
+def test_weights_are_equal_at_scales_of_nothing(dtype, prefix, bs, scale):
+    """Prefixes that end inside a tile: what is behind them has no weight, whatever the scale."""
+    torch.manual_seed(1)
+    new, keys, groups = [1, 2, 1], [prefix + 1, prefix + 20, prefix + 300], [(0, 3, prefix)]
+    for d, H, kvh in ((64, 4, 1), (128, 20, 2)):
+        cache, tables = pages(keys, groups, kvh, d, bs, dtype)
+        plan = K().SharedPrefixPlan(new, keys, groups, H, kvh, d, bs, device="cuda")
+        q = rand(4, H * d, dtype=dtype, std=2.0)
+        out = K().paged_attention_shared(q, torch.empty_like(q), cache, tables, plan, scale)
+        check(out, *attention_exact(q, cache, tables, new, keys, [prefix] * 3, H, scale))
