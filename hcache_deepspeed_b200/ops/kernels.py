@@ -975,7 +975,7 @@ def retention_stuck() -> bool:
 # ------------------------------------------------------------------------------------------------
 # (A step makes hundreds of these calls: their checks read each attribute once, and a stream is asked for by its number. A Stream object and
 # a device guard alone cost 5 us of the 22 that a call took; it takes 9 to 12 so.)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (a build of torch for the CPU alone has no such name, and no call)
 _I32, _F32, _LOGITS = torch.int32, torch.float32, (torch.bfloat16, torch.float16, torch.float32)
 
 

@@ -1,4 +1,7 @@
 """Batches of many requests at their edges, on the host: what plans keep alive, what the wrappers hand to the library and what they refuse."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
@@ -80,3 +83,13 @@ def test_a_plan_outlives_its_calls_on_other_streams(lib, call, args):
         call(**kw)
     assert len([c for c in lib.calls if c[0] in ("hds_adapter_add", "hds_paged_attention_shared")]) == 6
     assert kw["plan"]._dev.recorded == [7, 9]
+
+
+def test_the_package_imports_on_a_torch_without_cuda():
+    """A build of torch for the CPU alone has none of the ``_cuda_*`` names."""
+    gone = "import torch\nfor name in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, name)\n"
+    mods = ("hcache_deepspeed_b200", "hcache_deepspeed_b200.ops.kernels", "hcache_deepspeed_b200.models.transformer", "hcache_deepspeed_b200.models.hybrid",
+            "hcache_deepspeed_b200.linear", "hcache_deepspeed_b200.inference.sampling")
+    code = gone + "".join(f"import {m}\n" for m in mods) + "from hcache_deepspeed_b200.ops.plans import AdapterPlan\nAdapterPlan([0, -1], 1)\n"
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
