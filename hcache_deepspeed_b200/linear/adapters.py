@@ -14,7 +14,7 @@ from .optimized_linear import LoRAOptimizedLinear
 
 class AdapterBank(nn.Module):
     """``n`` adapters of a projection ``input_dim -> output_dim``, of up to ``rank`` each (rounded up to a multiple of 8; smaller ones are padded
-    with zeros). An adapter that was never loaded adds nothing."""
+    with zeros). An adapter that was never loaded adds nothing. Scales stay fp32 when the bank, or a module that has it, is converted."""
 
     def __init__(self, n: int, rank: int, input_dim: int, output_dim: int, device=None, dtype=torch.bfloat16):
         super().__init__()
@@ -24,6 +24,13 @@ class AdapterBank(nn.Module):
         self.register_buffer("down", torch.zeros(n, self.rank, input_dim, dtype=dtype, device=device))
         self.register_buffer("up", torch.zeros(n, output_dim, self.rank, dtype=dtype, device=device))
         self.register_buffer("scales", torch.zeros(n, dtype=torch.float32, device=device))
+
+    def _apply(self, fn, recurse=True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype != torch.float32:
+            self.scales = scales.to(self.scales.device)
+        return self
 
     @torch.no_grad()
     def load(self, i: int, down: torch.Tensor, up: torch.Tensor, scale: float) -> None:

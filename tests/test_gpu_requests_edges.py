@@ -52,3 +52,15 @@ def test_weights_are_equal_at_scales_of_nothing(dtype, prefix, bs, scale):
         q = rand(4, H * d, dtype=dtype, std=2.0)
         out = K().paged_attention_shared(q, torch.empty_like(q), cache, tables, plan, scale)
         check(out, *attention_exact(q, cache, tables, new, keys, [prefix] * 3, H, scale))
+
+
+def test_a_converted_bank_serves():
+    from hcache_deepspeed_b200.linear import AdapterBank, MultiAdapterLinear
+    torch.manual_seed(2)
+    bank = AdapterBank(2, 8, 64, 48, dtype=torch.float32)
+    for i in range(2):
+        bank.load(i, torch.randn(8, 64) / 8, torch.randn(48, 8), 1 / 3 + i)
+    layer = MultiAdapterLinear(torch.randn(48, 64) / 8, bank).to("cuda").to(torch.bfloat16)
+    ids, x = [1, -1, 0], rand(3, 64)
+    y = layer(x, bank.plan(ids))
+    check(y, *adapters_exact(K().gemm(x, layer.weight), x, bank.down, bank.up, bank.scales, ids))

@@ -5,6 +5,7 @@ import sys
 import pytest
 import torch
 
+from hcache_deepspeed_b200.linear import AdapterBank, MultiAdapterLinear
 from hcache_deepspeed_b200.ops import kernels, native, plans
 
 
@@ -93,3 +94,21 @@ def test_the_package_imports_on_a_torch_without_cuda():
     code = gone + "".join(f"import {m}\n" for m in mods) + "from hcache_deepspeed_b200.ops.plans import AdapterPlan\nAdapterPlan([0, -1], 1)\n"
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ---- banks of adapters ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("convert", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.float16),
+                                     lambda m: m.half().bfloat16()])
+def test_a_converted_bank_keeps_its_scales(convert):
+    """They are fp32 whatever the weights' type: nothing else is served, and 1 / 3 has other bits in 16."""
+    torch.manual_seed(0)
+    bank = AdapterBank(2, 8, 16, 24, dtype=torch.float32)
+    bank.load(1, torch.randn(8, 16), torch.randn(24, 8), 1 / 3)
+    layer = torch.nn.Sequential(MultiAdapterLinear(torch.randn(24, 16), bank))
+    kept = bank.scales.clone()
+    assert convert(layer) is layer and layer[0].bank is bank
+    assert bank.scales.dtype == torch.float32 and torch.equal(bank.scales, kept)
+    assert bank.down.dtype == bank.up.dtype == layer[0].weight.dtype != torch.float32
+    assert dict(bank.named_buffers())["scales"] is bank.scales and torch.equal(bank.state_dict()["scales"], kept)
+    bank.load(0, torch.randn(4, 16), torch.randn(24, 4), 0.7)
+    assert bank.scales[0] == torch.tensor(0.7)
