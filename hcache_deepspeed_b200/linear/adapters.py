@@ -39,6 +39,7 @@ class AdapterBank(nn.Module):
         if not 0 <= i < self.n or r > self.rank or tuple(down.shape) != (r, self.input_dim) or tuple(up.shape) != (self.output_dim, r):
             raise ValueError(f"adapter {i} of {self.n}: down {tuple(down.shape)}, up {tuple(up.shape)} do not fit rank {self.rank}, "
                              f"{self.input_dim} -> {self.output_dim}")
+        down, up = down.clone(), up.clone()       # (they may be rows of this bank, its own ones too)
         self.down[i].zero_()
         self.up[i].zero_()
         self.down[i, :r] = down

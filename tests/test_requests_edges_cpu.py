@@ -112,3 +112,17 @@ def test_a_converted_bank_keeps_its_scales(convert):
     assert dict(bank.named_buffers())["scales"] is bank.scales and torch.equal(bank.state_dict()["scales"], kept)
     bank.load(0, torch.randn(4, 16), torch.randn(24, 4), 0.7)
     assert bank.scales[0] == torch.tensor(0.7)
+
+
+def test_a_bank_loads_from_its_own_rows():
+    torch.manual_seed(1)
+    bank = AdapterBank(2, 16, 24, 40, dtype=torch.float32)
+    down, up = torch.randn(16, 24), torch.randn(40, 16)
+    bank.load(0, down, up, 1.0)
+    bank.load(0, bank.down[0], bank.up[0], 0.5)                          # another scale
+    assert torch.equal(bank.down[0], down) and torch.equal(bank.up[0], up) and bank.scales[0] == 0.5
+    bank.load(1, bank.down[0], bank.up[0], 2.0)                          # a copy
+    bank.load(0, bank.down[0, 3:10], bank.up[0, :, 3:10], 1.0)           # fewer ranks
+    assert torch.equal(bank.down[0, :7], down[3:10]) and torch.equal(bank.up[0, :, :7], up[:, 3:10])
+    assert not bank.down[0, 7:].any() and not bank.up[0, :, 7:].any()
+    assert torch.equal(bank.down[1], down) and torch.equal(bank.up[1], up)
