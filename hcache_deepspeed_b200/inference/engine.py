@@ -443,38 +443,42 @@ class InferenceEngine(torch.nn.Module):
         session_ids = kwargs.get("session_ids", None)
         ephemeral = session_ids is None
         Bsz = ids.shape[0]
+        from .sampling import LogitControls, sample_next
+        attention_mask = kwargs.get("attention_mask")
+        wanted = {k: kwargs[k] for k in ("repetition_penalty", "presence_penalty", "frequency_penalty", "logit_bias", "allowed") if kwargs.get(k) is not None}
+        controls = None
+        if wanted:       # (ahead of the prompt: what they refuse leaves no trace in the cache)
+            told = [ids[b] if attention_mask is None else ids[b][attention_mask[b].bool()] for b in range(Bsz)]
+            model = self._engine.model()
+            controls = LogitControls(told, model.spec.vocab, max_new, model.device, **wanted)
         if ephemeral:
             session_ids = [self._next_ephemeral_uid + i for i in range(Bsz)]
             self._next_ephemeral_uid += Bsz
-        from .sampling import LogitControls, sample_next
-        attention_mask = kwargs.get("attention_mask")
-        out = self._injected_forward(ids, session_ids=session_ids, last_token_only=True, attention_mask=attention_mask)
         seqs = [ids[b].tolist() for b in range(Bsz)]
-        wanted = {k: kwargs[k] for k in ("repetition_penalty", "presence_penalty", "frequency_penalty", "logit_bias", "allowed") if kwargs.get(k) is not None}
-        controls = None
-        if wanted:
-            told = [ids[b] if attention_mask is None else ids[b][attention_mask[b].bool()] for b in range(Bsz)]
-            controls = LogitControls(told, out.logits.shape[-1], max_new, out.logits.device, **wanted)
-        alive = list(range(Bsz))
-        for step in range(max_new):
-            nxt = sample_next(out.logits, do_sample, temperature, top_k, top_p, controls).cpu()
-            still, places = [], []
-            for j, b in enumerate(alive):
-                tok = int(nxt[j])
-                seqs[b].append(tok)
-                if tok not in eos_set:
-                    still.append((b, tok))
-                    places.append(j)
-            if not still or step == max_new - 1:
-                break
-            if controls is not None:
-                controls.keep(places)
-            alive = [b for b, _ in still]
-            step_ids = torch.tensor([[t] for _, t in still])
-            out = self._injected_forward(step_ids, session_ids=[session_ids[b] for b in alive], last_token_only=True)
-        if ephemeral:
-            for sid in session_ids:
-                self._engine.flush(sid)
+        try:
+            out = self._injected_forward(ids, session_ids=session_ids, last_token_only=True, attention_mask=attention_mask)
+            alive = list(range(Bsz))
+            for step in range(max_new):
+                nxt = sample_next(out.logits, do_sample, temperature, top_k, top_p, controls).cpu()
+                still, places = [], []
+                for j, b in enumerate(alive):
+                    tok = int(nxt[j])
+                    seqs[b].append(tok)
+                    if tok not in eos_set:
+                        still.append((b, tok))
+                        places.append(j)
+                if not still or step == max_new - 1:
+                    break
+                if controls is not None:
+                    controls.keep(places)
+                alive = [b for b, _ in still]
+                step_ids = torch.tensor([[t] for _, t in still])
+                out = self._injected_forward(step_ids, session_ids=[session_ids[b] for b in alive], last_token_only=True)
+        finally:
+            if ephemeral:
+                for sid in session_ids:
+                    if self._engine.state_manager.get_sequence(sid) is not None:       # (not there where the prompt was refused)
+                        self._engine.flush(sid)
         width = max(len(s) for s in seqs)
         pad = getattr(getattr(self.module, "config", None), "pad_token_id", None)
         pad = pad if pad is not None else (next(iter(eos_set)) if eos_set else 0)

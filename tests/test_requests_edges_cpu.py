@@ -126,3 +126,52 @@ def test_a_bank_loads_from_its_own_rows():
     assert torch.equal(bank.down[0, :7], down[3:10]) and torch.equal(bank.up[0, :, :7], up[:, 3:10])
     assert not bank.down[0, 7:].any() and not bank.up[0, :, 7:].any()
     assert torch.equal(bank.down[1], down) and torch.equal(bank.up[1], up)
+
+
+# ---- generate under controls ---------------------------------------------------------------------------------------------
+def small_engine():
+    transformers = pytest.importorskip("transformers")
+    import hcache_deepspeed_b200 as ds
+    torch.manual_seed(0)
+    cfg = transformers.LlamaConfig(vocab_size=128, hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                                   max_position_embeddings=256)
+    return ds.init_inference(transformers.LlamaForCausalLM(cfg).eval(), dtype=torch.float32, replace_with_kernel_inject=True)
+
+
+REFUSED = [dict(logit_bias={128: 1.0}), dict(logit_bias=[{}]), dict(repetition_penalty=0.0), dict(presence_penalty=[1.0, 2.0, 3.0]),
+           dict(allowed=torch.ones(2, 127, dtype=torch.bool)), dict(frequency_penalty=float("nan"))]
+
+
+def test_a_refused_request_leaves_nothing_behind():
+    eng = small_engine()
+    state = eng.ragged_engine.state_manager
+    ids = torch.randint(3, 128, (2, 9))
+    free, tracked = int(state.free_blocks[0]), state.n_tracked_sequences
+    for kw in REFUSED:
+        with pytest.raises(ValueError):
+            eng.generate(input_ids=ids, max_new_tokens=4, **kw)
+        assert (int(state.free_blocks[0]), state.n_tracked_sequences) == (free, tracked)
+    want = eng.generate(input_ids=ids, max_new_tokens=4, repetition_penalty=1.5)
+    for kw in REFUSED:          # a session is as it was: the same prompt, asked again without the mistake, has the same answer
+        with pytest.raises(ValueError):
+            eng.generate(input_ids=ids, max_new_tokens=4, session_ids=[5, 6], **kw)
+    assert torch.equal(eng.generate(input_ids=ids, max_new_tokens=4, session_ids=[5, 6], repetition_penalty=1.5), want)
+    assert state.get_sequence(5).seen_tokens == 9 + 3
+
+
+def test_a_request_that_fails_on_its_way_leaves_nothing_behind(monkeypatch):
+    eng = small_engine()
+    state = eng.ragged_engine.state_manager
+    free, tracked = int(state.free_blocks[0]), state.n_tracked_sequences
+    from hcache_deepspeed_b200.inference import sampling
+    calls, plain = [], sampling.sample_next
+
+    def failing(*args):
+        calls.append(1)
+        if len(calls) == 3:
+            raise KeyboardInterrupt
+        return plain(*args)
+    monkeypatch.setattr(sampling, "sample_next", failing)
+    with pytest.raises(KeyboardInterrupt):
+        eng.generate(input_ids=torch.randint(3, 128, (2, 9)), max_new_tokens=4, logit_bias={3: 1.0})
+    assert (int(state.free_blocks[0]), state.n_tracked_sequences) == (free, tracked)
