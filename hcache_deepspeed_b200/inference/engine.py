@@ -79,6 +79,7 @@ class InferenceEngine(torch.nn.Module):
         self._graph_output = None
         self._sessions_latents: Dict[int, List[torch.Tensor]] = {}
         self._sessions_tokens: Dict[int, List[torch.Tensor]] = {}
+        self._context: Dict[int, List[int]] = {}       # the tokens that a session has in the KV cache
         self._next_ephemeral_uid = 1 << 40
         self._engine = None
         if config.enable_cuda_graph and config.tensor_parallel.tp_size > 1:
@@ -245,14 +246,21 @@ class InferenceEngine(torch.nn.Module):
         self._engine.restore_kv([session_id], [tokens.reshape(-1)], [latents])
         self._sessions_latents[session_id] = [latents]
         self._sessions_tokens[session_id] = [tokens.reshape(-1).cpu()]
+        self._context[session_id] = tokens.reshape(-1).tolist()
 
     def flush(self, session_id: int, drop_hidden_states: bool = False) -> None:
         """Drop a session's KV cache (its saved hidden states survive unless ``drop_hidden_states``)."""
         self._require_injected()
         self._engine.flush(session_id)
+        self._context.pop(session_id, None)
         if drop_hidden_states:
             self._sessions_latents.pop(session_id, None)
             self._sessions_tokens.pop(session_id, None)
+
+    def _context_of(self, session_id: int) -> List[int]:
+        """The tokens ahead of a session's next one, where all of them came through this engine (and not through :attr:`ragged_engine`)."""
+        seq, told = self._engine.state_manager.get_sequence(session_id), self._context.get(session_id, [])
+        return told if seq is not None and seq.seen_tokens == len(told) else []
 
     def _require_injected(self) -> None:
         if self._engine is None:
@@ -283,6 +291,11 @@ class InferenceEngine(torch.nn.Module):
         if ephemeral:
             for sid in session_ids:
                 self._engine.flush(sid)
+        else:
+            for sid, row in zip(session_ids, rows):
+                if self._engine.state_manager.get_sequence(sid).seen_tokens == row.numel():
+                    self._context[sid] = []       # (the session begins: an earlier one of its number ended elsewhere)
+                self._context.setdefault(sid, []).extend(row.tolist())
         if not last_token_only:
             if all(r.numel() == T for r in rows):
                 logits = logits.view(Bsz, T, -1)
@@ -416,7 +429,8 @@ class InferenceEngine(torch.nn.Module):
     def generate(self, *inputs, **kwargs):
         """Injected: greedy / temperature / top-k / top-p sampling over sessions, under ``repetition_penalty``, ``presence_penalty``,
         ``frequency_penalty`` (numbers, or lists with one per row), ``logit_bias`` (a dict, or a list of them) and ``allowed`` (bool
-        ``[rows, vocab]``), see :class:`LogitControls`. Otherwise HF ``generate`` (``num_beams > 1`` is rejected exactly as in the reference,
+        ``[rows, vocab]``, the same for every step), see :class:`LogitControls`. To penalties, what a session has in the KV cache already is part of the
+        prompt, its own answers too (unless it got some of it through :attr:`ragged_engine`: then it is this call's tokens alone). Otherwise HF ``generate`` (``num_beams > 1`` is rejected exactly as in the reference,
         engine.py:583-606)."""
         num_beams = kwargs.get("num_beams", 1)
         gc = kwargs.get("generation_config", None)
@@ -449,6 +463,8 @@ class InferenceEngine(torch.nn.Module):
         controls = None
         if wanted:       # (ahead of the prompt: what they refuse leaves no trace in the cache)
             told = [ids[b] if attention_mask is None else ids[b][attention_mask[b].bool()] for b in range(Bsz)]
+            if not ephemeral:
+                told = [self._context_of(sid) + t.tolist() for sid, t in zip(session_ids, told)]
             model = self._engine.model()
             controls = LogitControls(told, model.spec.vocab, max_new, model.device, **wanted)
         if ephemeral:
@@ -477,6 +493,7 @@ class InferenceEngine(torch.nn.Module):
         finally:
             if ephemeral:
                 for sid in session_ids:
+                    self._context.pop(sid, None)
                     if self._engine.state_manager.get_sequence(sid) is not None:       # (not there where the prompt was refused)
                         self._engine.flush(sid)
         width = max(len(s) for s in seqs)

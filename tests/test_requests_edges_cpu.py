@@ -175,3 +175,59 @@ def test_a_request_that_fails_on_its_way_leaves_nothing_behind(monkeypatch):
     with pytest.raises(KeyboardInterrupt):
         eng.generate(input_ids=torch.randint(3, 128, (2, 9)), max_new_tokens=4, logit_bias={3: 1.0})
     assert (int(state.free_blocks[0]), state.n_tracked_sequences) == (free, tracked)
+
+
+PENALTIES = dict(repetition_penalty=1.9, presence_penalty=0.3, frequency_penalty=[0.2, 0.0])
+
+
+def test_a_sessions_earlier_turns_count():
+    """Two turns give what one call with all of their tokens gives."""
+    eng = small_engine()
+    ids = torch.randint(3, 128, (2, 9))
+    first = eng.generate(input_ids=ids, max_new_tokens=5, session_ids=[5, 6])
+    more = torch.cat([first[:, -1:], torch.randint(3, 128, (2, 4))], 1)       # (the last token of an answer has not been fed yet)
+    want = eng.generate(input_ids=torch.cat([first[:, :-1], more], 1), max_new_tokens=12, **PENALTIES)
+    plain = eng.generate(input_ids=torch.cat([first[:, :-1], more], 1), max_new_tokens=12)
+    got = eng.generate(input_ids=more, max_new_tokens=12, session_ids=[5, 6], **PENALTIES)
+    assert torch.equal(got, want[:, first.shape[1] - 1:]) and not torch.equal(want, plain)
+    third = torch.cat([got[:, -1:], torch.randint(3, 128, (2, 2))], 1)        # a third turn, with the answer given under penalties behind it
+    want = eng.generate(input_ids=torch.cat([first[:, :-1], got[:, :-1], third], 1), max_new_tokens=6, **PENALTIES)
+    assert torch.equal(eng.generate(input_ids=third, max_new_tokens=6, session_ids=[5, 6], **PENALTIES)[:, 3:], want[:, -6:])
+
+
+def test_a_session_that_was_dropped_begins_anew():
+    eng = small_engine()
+    ids, other = torch.randint(3, 128, (2, 9)), torch.randint(3, 128, (2, 7))
+    want = eng.generate(input_ids=other, max_new_tokens=8, **PENALTIES)
+    for drop in (eng.flush, eng.ragged_engine.flush):
+        eng.generate(input_ids=ids, max_new_tokens=5, session_ids=[5, 6])
+        for sid in (5, 6):
+            drop(sid)
+        assert torch.equal(eng.generate(input_ids=other, max_new_tokens=8, session_ids=[5, 6], **PENALTIES), want)
+        for sid in (5, 6):
+            eng.flush(sid)
+    eng.ragged_engine.put([5, 6], list(ids))       # tokens that this engine has not seen: the call's own count
+    eng.generate(input_ids=other, max_new_tokens=2, session_ids=[5, 6], **PENALTIES)
+    assert eng._context_of(5) == []
+    for sid in (5, 6):
+        eng.flush(sid)
+    assert not eng._context
+
+
+def test_a_restored_sessions_earlier_turns_count():
+    import hcache_deepspeed_b200 as ds
+    transformers = pytest.importorskip("transformers")
+    torch.manual_seed(0)
+    cfg = transformers.LlamaConfig(vocab_size=128, hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                                   max_position_embeddings=256)
+    eng = ds.init_inference(transformers.LlamaForCausalLM(cfg).eval(), dtype=torch.float32, replace_with_kernel_inject=True, hcache={"enabled": True})
+    more = torch.randint(3, 128, (1, 4))
+    ids = eng.generate(input_ids=more, max_new_tokens=40)[:, 4:]       # what this model likes to say
+    kw = dict(repetition_penalty=3.0)
+    eng.forward(ids, session_ids=[5])
+    tokens, latents = eng.session_tokens(5), eng.hidden_states(5)
+    eng.flush(5)
+    eng.restore_hidden_states(5, tokens, latents)
+    got = eng.generate(input_ids=more, max_new_tokens=20, session_ids=[5], **kw)
+    want = eng.generate(input_ids=torch.cat([ids, more], 1), max_new_tokens=20, **kw)
+    assert torch.equal(got, want[:, ids.shape[1]:])
