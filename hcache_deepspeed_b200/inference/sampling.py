@@ -18,7 +18,7 @@ def pack_mask(allowed: torch.Tensor) -> torch.Tensor:
 
 class LogitControls:
     """What the requests of a batch lay on their logits from step to step: penalties for repeated tokens, a bias per token, a mask of the
-    tokens that a grammar allows next. ``prompts[i]``: the tokens of request i so far; numbers and dicts are for all requests, lists of them for
+    tokens that a grammar allows next. ``prompts[i]``: the tokens of request i so far (of a session, its earlier turns' too); numbers and dicts are for all requests, lists of them for
     each. ``ops.kernels.logit_controls`` has the formulas."""
 
     def __init__(self, prompts: Sequence, vocab: int, max_new_tokens: int, device, repetition_penalty: Union[float, Sequence[float]] = 1.0,
@@ -29,9 +29,9 @@ class LogitControls:
         each = lambda v, name: self._each(v, n, name)  # noqa: E731
         rep, pres, freq = each(repetition_penalty, "repetition_penalty"), each(presence_penalty, "presence_penalty"), each(frequency_penalty, "frequency_penalty")
         if any(not 0 < r < math.inf for r in rep):
-            raise ValueError("repetition_penalty must be positive and finite")
+            raise ValueError("repetition_penalty must be positive and finite in 32 bits")
         if not all(map(math.isfinite, pres + freq)):
-            raise ValueError("presence_penalty and frequency_penalty must be finite")
+            raise ValueError("presence_penalty and frequency_penalty must be finite in 32 bits")
         self._c = {}
         self._room = 0
         if any(r != 1 for r in rep) or any(pres) or any(freq):
@@ -50,10 +50,10 @@ class LogitControls:
             k = max(map(len, lists), default=0)
             if any(not 0 <= t < vocab for b in lists for t in b):
                 raise ValueError("logit_bias names a token outside the vocabulary")
-            if any(not v < math.inf for b in lists for v in b.values()):
-                raise ValueError("logit_bias must be finite, or -inf")
-            self._c["bias_ids"] = torch.tensor([list(b) + [-1] * (k - len(b)) for b in lists], dtype=torch.int32).reshape(n, k)
-            self._c["bias"] = torch.tensor([list(b.values()) + [0.0] * (k - len(b)) for b in lists], dtype=torch.float32).reshape(n, k)
+            bias = torch.tensor([list(b.values()) + [0.0] * (k - len(b)) for b in lists], dtype=torch.float32).reshape(n, k)
+            if not (bias < math.inf).all():
+                raise ValueError("logit_bias must be finite in 32 bits, or -inf")
+            self._c["bias_ids"], self._c["bias"] = torch.tensor([list(b) + [-1] * (k - len(b)) for b in lists], dtype=torch.int32).reshape(n, k), bias
         self._c = {name: t.to(self.device) for name, t in self._c.items()}
         self.n = n
         self.set_allowed(allowed)
@@ -63,7 +63,7 @@ class LogitControls:
         values = [float(v) for v in value] if isinstance(value, (list, tuple)) else [float(value)] * n
         if len(values) != n:
             raise ValueError(f"{name} is for {len(values)} requests, there are {n}")
-        return values
+        return torch.tensor(values, dtype=torch.float32).tolist()       # as the kernel has them: 1e39 is infinite, 1e-46 nothing
 
     def set_allowed(self, allowed: Optional[torch.Tensor]) -> None:
         """The tokens that may come next: bool ``[n, vocab]``, or None for all. Stays until the next call."""

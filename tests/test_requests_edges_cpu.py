@@ -5,6 +5,7 @@ import sys
 import pytest
 import torch
 
+from hcache_deepspeed_b200.inference.sampling import LogitControls, sample_next
 from hcache_deepspeed_b200.linear import AdapterBank, MultiAdapterLinear
 from hcache_deepspeed_b200.ops import kernels, native, plans
 
@@ -231,3 +232,18 @@ def test_a_restored_sessions_earlier_turns_count():
     got = eng.generate(input_ids=more, max_new_tokens=20, session_ids=[5], **kw)
     want = eng.generate(input_ids=torch.cat([ids, more], 1), max_new_tokens=20, **kw)
     assert torch.equal(got, want[:, ids.shape[1]:])
+
+
+# ---- controls on logits --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(repetition_penalty=1e39), dict(repetition_penalty=[1.0, 1e-46]), dict(presence_penalty=1e39), dict(frequency_penalty=[-1e39, 0.0]),
+                                dict(logit_bias={3: 1e39}), dict(logit_bias=[{}, {8: 4e38}])])
+def test_controls_refuse_what_is_no_number_in_32_bits(kw):
+    """The kernel has them in 32 bits, where 1e39 is infinite and 1e-46 is 0: logits of 0 times or by these are NaN."""
+    with pytest.raises(ValueError, match="32 bits"):
+        LogitControls([[1], [2]], 9, 3, "cpu", **kw)
+
+
+def test_controls_at_the_ends_of_32_bits():
+    controls = LogitControls([[1, 2]], 4, 3, "cpu", repetition_penalty=3e38, presence_penalty=-1e-30, logit_bias={3: -1e39})
+    assert controls.apply(torch.tensor([[1.0, 0.0, -1.0, 1.0]])).tolist() == [[1.0, 0.0, torch.tensor(-3e38).item(), float("-inf")]]
+    assert sample_next(torch.tensor([[1.0, 0.0, -1.0, 1.0]]), controls=controls).tolist() == [0]
