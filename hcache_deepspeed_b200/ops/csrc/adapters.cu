@@ -652,6 +652,7 @@ extern "C" int hds_adapter_add(const void* base, int64_t ld_base, const void* x,
                 "adapter_add: widths are multiples of 8 below 2^24");
     HDS_REQUIRE(ld_base % 8 == 0 && ld_x % 8 == 0 && ld_out % 8 == 0, "adapter_add: rows start on 16-byte boundaries");
     HDS_REQUIRE(ld_base >= 0 && ld_x >= 0 && ld_out >= 0 && ld_base < (1 << 30) && ld_x < (1 << 30) && ld_out < (1 << 30), "adapter_add: rows are less than 2^30 apart");
+    HDS_REQUIRE(rows <= 1 || ld_out >= outputs, "adapter_add: rows of out share memory");
     HDS_REQUIRE(((reinterpret_cast<uintptr_t>(base) | reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(down) |
                   reinterpret_cast<uintptr_t>(up) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(tiles)) & 15) == 0,
                 "adapter_add: operands start on 16-byte boundaries");

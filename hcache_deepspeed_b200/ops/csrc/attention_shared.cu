@@ -762,6 +762,8 @@ extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out
     if (rows == 0 || n_workers == 0) return HDS_OK;
     HDS_REQUIRE(ld_q % 8 == 0 && ld_out % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
                 "paged_attention_shared: rows start on 16-byte boundaries");
+    HDS_REQUIRE(rows <= 1 || (ld_q >= static_cast<int64_t>(n_q_heads) * head_dim && ld_out >= static_cast<int64_t>(n_q_heads) * head_dim),
+                "paged_attention_shared: rows of q or out share memory");
     HDS_REQUIRE(((reinterpret_cast<uintptr_t>(tiles) | reinterpret_cast<uintptr_t>(items) | reinterpret_cast<uintptr_t>(workers)) & 15) == 0 &&
                     (reinterpret_cast<uintptr_t>(units) & 7) == 0,
                 "paged_attention_shared: unaligned work lists");

@@ -304,6 +304,7 @@ extern "C" int hds_logit_controls(const void* logits, int64_t ld_logits, void* o
     HDS_REQUIRE(n_bias >= 0 && capacity >= 0 && capacity < (1 << 30) && n_masks >= 0, "logit_controls: sizes in [0, 2^30)");
     HDS_REQUIRE(history == nullptr || history_len != nullptr, "logit_controls: a history needs its lengths");
     HDS_REQUIRE(mask == nullptr || ld_mask >= (static_cast<int64_t>(vocab) + 31) / 32, "logit_controls: a mask has a bit per token");
+    HDS_REQUIRE(rows <= 1 || ld_out >= vocab, "logit_controls: rows of out share memory");
     const int elem = dtype == 2 ? 4 : 2;
     HDS_REQUIRE(reinterpret_cast<uintptr_t>(logits) % elem == 0 && reinterpret_cast<uintptr_t>(out) % elem == 0, "logit_controls: logits on odd addresses");
     if (rows == 0 || vocab == 0) return HDS_OK;

@@ -1008,6 +1008,14 @@ def _rows(t: torch.Tensor, name: str) -> int:
     return st[0] if shape[0] > 1 else shape[1]
 
 
+def _rows_apart(t: torch.Tensor, name: str) -> int:
+    """The same where no two rows may share memory: of a tensor that is written, or that tensor maps describe."""
+    ld, (rows, width) = _rows(t, name), t.shape
+    if ld < width and rows > 1:
+        raise ValueError(f"rows of {name} share memory: {(rows, width)} / {t.stride()}")
+    return ld
+
+
 @functools.lru_cache(maxsize=1024)
 def _adapter_parts(index: int, tiles: int, width: int) -> int:
     return native.cuda_lib().hds_adapter_parts(tiles, width)       # (of the current device, which is number `index`)
@@ -1037,7 +1045,7 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
     if out is None:
         out, ld_out = x.new_empty((T, N)), N
     else:
-        ld_out = _rows(out, "out")
+        ld_out = _rows_apart(out, "out")
         if out.shape != (T, N) or out.dtype != dtype:
             raise ValueError("out must be like base")
     if not index == base.get_device() == down.get_device() == up.get_device() == scales.get_device() == out.get_device():
@@ -1069,10 +1077,10 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     """Causal attention of a batch whose sequences share prefixes (``plan``), each prefix read once for its group. ``q`` and ``out``
     [rows, n_q_heads * head_dim], a sequence's new tokens being neighbouring rows in the plan's order; rows behind the last sequence are left as they
     are. ``kv_cache_layer`` [blocks, 2, n_kv_heads, block_size, head_dim] holds the new tokens' keys already; ``block_tables`` int32
-    [sequences, stride]. head_dim 64 or 128, 16-bit. A group's pages are those that its first sequence's table names. Finite ``scale`` of 0 or more.
+    [sequences, stride]. head_dim 64 or 128, 16-bit. ``out`` may be ``q``, and overlaps no operand otherwise. A group's pages are those that its first sequence's table names. Finite ``scale`` of 0 or more.
     The call allocates its scratch."""
     index, cache = _place(q, "q"), kv_cache_layer.shape
-    ld_q, ld_out, dt, dtype = _rows(q, "q"), _rows(out, "out"), _dt(q), q.dtype
+    ld_q, ld_out, dt, dtype = _rows_apart(q, "q"), _rows_apart(out, "out"), _dt(q), q.dtype
     d, H, rows = plan.head_dim, plan.n_q_heads, plan.rows
     if d not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {d}")
@@ -1130,7 +1138,7 @@ def _check_controls(logits: torch.Tensor, out: torch.Tensor, history, history_le
                     mask_rows) -> Tuple[int, ...]:
     """What :func:`logit_controls` takes, and the restatement in torch: elements between the rows of logits, out, history, bias_ids, bias and mask;
     history places, biases and masks."""
-    ld, ld_out, shape, dtype, index = _rows(logits, "logits"), _rows(out, "out"), logits.shape, logits.dtype, logits.get_device()
+    ld, ld_out, shape, dtype, index = _rows(logits, "logits"), _rows_apart(out, "out"), logits.shape, logits.dtype, logits.get_device()
     n, V = shape
     if dtype not in _LOGITS:
         raise TypeError(f"unsupported logits dtype {dtype}: bf16, fp16 or fp32")
@@ -1183,7 +1191,8 @@ def logit_controls(logits: torch.Tensor, out: Optional[torch.Tensor] = None, *, 
                    history_len: Optional[torch.Tensor] = None, prompt_len: Optional[torch.Tensor] = None, repetition: Optional[torch.Tensor] = None,
                    presence: Optional[torch.Tensor] = None, frequency: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
                    bias: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, mask_rows: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """What every row's request lays on its logits ``[n, vocab]``, in this order (``out`` may be ``logits``):
+    """What every row's request lays on its logits ``[n, vocab]``, in this order (``out`` may be ``logits``, and
+    overlaps no operand otherwise):
 
     ``repetition`` fp32 [n]: logits of tokens in the row's history are divided by it where positive, multiplied where not; ``frequency`` and
     ``presence`` fp32 [n]: taken off once per time that the token stands in the answer, and once if it does. ``history`` int32 [n, places] holds

@@ -87,6 +87,37 @@ def test_a_plan_outlives_its_calls_on_other_streams(lib, call, args):
     assert kw["plan"]._dev.recorded == [7, 9]
 
 
+def controls_call(n=3, V=40):
+    return dict(logits=gpu(torch.zeros(n, V)))
+
+
+WRAPPERS = [(kernels.adapter_add, adapters_call, (3, 8), torch.bfloat16), (kernels.paged_attention_shared, shared_call, (2, 128), torch.bfloat16),
+            (kernels.logit_controls, controls_call, (3, 40), torch.float32)]
+
+
+@pytest.mark.parametrize("call,args,shape,dtype", WRAPPERS)
+def test_outputs_whose_rows_share_memory_are_refused(lib, call, args, shape, dtype):
+    """Two rows of them would be written to the same place, in any order. (A tensor map of the queries has no room for such rows either.)"""
+    memory = torch.zeros(4 * shape[1], dtype=dtype)
+    for name in ("out", "q") if call is kernels.paged_attention_shared else ("out", ):
+        for stride in (0, 1, shape[1] - 1):
+            with pytest.raises(ValueError, match="share memory"):
+                call(**{**args(), name: gpu(memory.as_strided(shape, (stride, 1)))})
+        assert not lib.calls
+        call(**{**args(), name: gpu(memory.as_strided(shape, (shape[1], 1)))})
+        assert len(lib.calls) >= 1
+        lib.calls.clear()
+
+
+@pytest.mark.parametrize("call,args,shape,dtype", WRAPPERS)
+def test_inputs_may_be_one_row_for_all(lib, call, args, shape, dtype):
+    kw = args()
+    for name in {"adapter_add": ("base", "x"), "paged_attention_shared": ("block_tables", ), "logit_controls": ("logits", )}[call.__name__]:
+        kw[name] = gpu(kw[name][:1].as_subclass(torch.Tensor).expand(kw[name].shape))
+    call(**kw)
+    assert len(lib.calls) >= 1
+
+
 def test_the_package_imports_on_a_torch_without_cuda():
     """A build of torch for the CPU alone has none of the ``_cuda_*`` names."""
     gone = "import torch\nfor name in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, name)\n"
