@@ -1038,8 +1038,8 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: tor
                          f"scales {tuple(scales.shape)}")
     if base.dtype != dtype or down.dtype != dtype or up.dtype != dtype or scales.dtype != torch.float32 or not scales.is_contiguous():
         raise TypeError("base, x, down and up have one type, scales are contiguous fp32")
-    if R % 8 or not 8 <= R <= 256 or K % 8 or N % 8 or not K or not N:
-        raise ValueError(f"K, N and the rank are multiples of 8, the rank at most 256; got {K}, {N}, {R}")
+    if R % 8 or not 8 <= R <= 256 or K % 8 or N % 8 or not 0 < K < 1 << 24 or not 0 < N < 1 << 24:
+        raise ValueError(f"K, N and the rank are multiples of 8, the rank at most 256, K and N below 2^24; got {K}, {N}, {R}")
     if plan.n_rows != T or plan.n_adapters != n:
         raise ValueError(f"the plan is for {plan.n_rows} rows of {plan.n_adapters} adapters, the call has {T} of {n}")
     if out is None:
@@ -1093,8 +1093,9 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     if cache != (blocks, 2, plan.n_kv_heads, plan.block_size, d) or not kv_cache_layer.is_contiguous():
         raise ValueError(f"the cache must be contiguous [blocks, 2, {plan.n_kv_heads}, {plan.block_size}, {d}], got {tuple(cache)}")
     ld_tables, (n_tables, width) = _rows(block_tables, "block_tables"), block_tables.shape
-    if block_tables.dtype != torch.int32 or n_tables < plan.n_seqs or width < plan.max_blocks:
-        raise ValueError(f"block_tables must be int32 [{plan.n_seqs}, at least {plan.max_blocks}], got {block_tables.dtype} {tuple(block_tables.shape)}")
+    if block_tables.dtype != torch.int32 or n_tables < plan.n_seqs or width < plan.max_blocks or ld_tables >= 1 << 31:
+        raise ValueError(f"block_tables must be int32 [{plan.n_seqs}, at least {plan.max_blocks}], rows less than 2^31 apart, got {block_tables.dtype} "
+                         f"{tuple(block_tables.shape)} / {block_tables.stride()}")
     if not index == out.get_device() == kv_cache_layer.get_device() == block_tables.get_device():
         _elsewhere(index, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
     if plan.index != index:
@@ -1181,6 +1182,8 @@ def _check_controls(logits: torch.Tensor, out: torch.Tensor, history, history_le
         here = here and mask.get_device() == index and (mask_rows is None or mask_rows.get_device() == index)
     elif mask_rows is not None:
         raise ValueError("mask_rows needs masks")
+    if places >= 1 << 30 or n_bias >= 1 << 30 or n_masks >= 1 << 30:       # (the library takes them as 32-bit numbers)
+        raise ValueError("histories, biases and masks: fewer than 2^30")
     if not here:
         _elsewhere(index, out=out, history=history, history_len=history_len, prompt_len=prompt_len, repetition=repetition, presence=presence,
                    frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, mask_rows=mask_rows)

@@ -118,6 +118,26 @@ def test_inputs_may_be_one_row_for_all(lib, call, args, shape, dtype):
     assert len(lib.calls) >= 1
 
 
+def test_sizes_that_the_library_takes_in_32_bits_are_refused_beyond(lib):
+    """(Address space alone: nobody touches these tensors.)"""
+    space = lambda shape, strides, dtype: gpu(torch.empty_strided(shape, strides, dtype=dtype))  # noqa: E731
+    i32, f32, bf = torch.int32, torch.float32, torch.bfloat16
+    with pytest.raises(ValueError, match="2.31 apart"):
+        kernels.paged_attention_shared(**{**shared_call(), "block_tables": space((2, 3), (1 << 31, 1), i32)})
+    lengths = gpu(torch.zeros(1, dtype=i32))
+    wide = dict(shape=(1, 1 << 30), strides=(1 << 30, 1))
+    for kw in (dict(history=space(**wide, dtype=i32), history_len=lengths), dict(bias_ids=space(**wide, dtype=i32), bias=space(**wide, dtype=f32)),
+               dict(mask=space((1 << 30, 2), (0, 1), i32), mask_rows=lengths)):
+        with pytest.raises(ValueError, match="fewer than 2.30"):
+            kernels.logit_controls(**controls_call(1), **kw)
+    for K, N in ((1 << 24, 8), (8, 1 << 24)):
+        kw = {**adapters_call(1, 1), "base": space((1, N), (N, 1), bf), "x": space((1, K), (K, 1), bf), "down": space((1, 8, K), (8 * K, K, 1), bf),
+              "up": space((1, N, 8), (8 * N, 8, 1), bf)}
+        with pytest.raises(ValueError, match="below 2.24"):
+            kernels.adapter_add(**kw)
+    assert not lib.calls
+
+
 def test_the_package_imports_on_a_torch_without_cuda():
     """A build of torch for the CPU alone has none of the ``_cuda_*`` names."""
     gone = "import torch\nfor name in [n for n in dir(torch._C) if n.startswith('_cuda_')]: delattr(torch._C, name)\n"
