@@ -16,6 +16,7 @@ import torch
 
 from . import reference as ref
 from .fp8 import Fp8Weight, quantize_rows_reference
+from .plans import MAX_SCALE
 
 
 def _fp8_emulate(a, w):
@@ -266,8 +267,8 @@ class CpuOps:
         return out
 
     def attention_shared(self, q, out, kv_layer, block_tables, plan, scale):
-        if not 0.0 <= scale < float("inf"):
-            raise ValueError(f"scale must be finite and not negative, got {scale}")
+        if not 0.0 <= scale < MAX_SCALE:
+            raise ValueError(f"scale must be below 2^127 and not negative, got {scale}")
         T, d = plan.rows, plan.head_dim
         items = torch.tensor([(i, r, n, k - n) for (i, r, n, k) in plan.items[:, :4].tolist() if n], dtype=torch.int32)
         if T:

@@ -757,7 +757,7 @@ extern "C" int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out
                 "paged_attention_shared: up to 128 query heads per KV head");
     HDS_REQUIRE(dtype == 0 || dtype == 1, "paged_attention_shared: dtype must be 0 (bf16) or 1 (fp16)");
     HDS_REQUIRE(p_splits >= 1 && p_splits <= 64, "paged_attention_shared: 1 to 64 splits of the prefix");
-    HDS_REQUIRE(scale >= 0.0f && scale < INFINITY, "paged_attention_shared: scale must be finite and not negative");      // (maxima are of raw scores)
+    HDS_REQUIRE(scale >= 0.0f && scale < 0x1p127f, "paged_attention_shared: scale must be below 2^127 and not negative");      // (maxima are of raw scores)
     HDS_REQUIRE(n_tiles >= 0 && rows >= 0 && n_workers >= 0 && n_units >= 0, "paged_attention_shared: negative size");
     if (rows == 0 || n_workers == 0) return HDS_OK;
     HDS_REQUIRE(ld_q % 8 == 0 && ld_out % 8 == 0 && ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,

@@ -14,13 +14,12 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
-import math
 from typing import Optional, Sequence, Tuple
 
 import torch
 
 from . import native
-from .plans import ADAPTER_FEW, AdapterPlan, SharedPrefixPlan  # noqa: F401
+from .plans import ADAPTER_FEW, MAX_SCALE, AdapterPlan, SharedPrefixPlan  # noqa: F401
 
 ACT_IDENTITY, ACT_GELU, ACT_RELU, ACT_SILU, ACT_GELU_TANH, ACT_SWIGLU_CLAMPED, ACT_RELU2 = 0, 1, 2, 3, 4, 5, 6
 ACT_CODES = {"identity": 0, None: 0, "gelu": 1, "relu": 2, "silu": 3, "gelu_tanh": 4, "gelu_new": 4,
@@ -1077,7 +1076,7 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
     """Causal attention of a batch whose sequences share prefixes (``plan``), each prefix read once for its group. ``q`` and ``out``
     [rows, n_q_heads * head_dim], a sequence's new tokens being neighbouring rows in the plan's order; rows behind the last sequence are left as they
     are. ``kv_cache_layer`` [blocks, 2, n_kv_heads, block_size, head_dim] holds the new tokens' keys already; ``block_tables`` int32
-    [sequences, stride]. head_dim 64 or 128, 16-bit. ``out`` may be ``q``, and overlaps no operand otherwise. A group's pages are those that its first sequence's table names. Finite ``scale`` of 0 or more.
+    [sequences, stride]. head_dim 64 or 128, 16-bit. ``out`` may be ``q``, and overlaps no operand otherwise. A group's pages are those that its first sequence's table names. ``scale`` from 0 to below 2^127.
     The call allocates its scratch."""
     index, cache = _place(q, "q"), kv_cache_layer.shape
     ld_q, ld_out, dt, dtype = _rows_apart(q, "q"), _rows_apart(out, "out"), _dt(q), q.dtype
@@ -1100,8 +1099,8 @@ def paged_attention_shared(q: torch.Tensor, out: torch.Tensor, kv_cache_layer: t
         _elsewhere(index, out=out, kv_cache_layer=kv_cache_layer, block_tables=block_tables)
     if plan.index != index:
         raise ValueError(f"the plan is on {plan.device}, the call is on cuda:{index}")
-    if not 0.0 <= scale < math.inf:
-        raise ValueError(f"scale must be finite and not negative, got {scale}")
+    if not 0.0 <= scale < MAX_SCALE:
+        raise ValueError(f"scale must be below 2^127 and not negative, got {scale}")
     if rows == 0:
         return out
     lib = native.cuda_lib()

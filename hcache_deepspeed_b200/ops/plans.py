@@ -16,6 +16,8 @@ OWN_ROWS, OWN_STRIP = 8, 16
 OWN_WORKERS, OWN_BEGIN = 12, 2
 #: microseconds: an SM's for a strip of own keys, a CTA's for 128 keys of a prefix under one and under two tiles of rows (measured, see attention_shared.cu)
 T_OWN, T_ONE, T_TWO = 0.17, 1.3, 2.9
+#: of attention's scores: times log2(e) it has to be a number in 32 bits
+MAX_SCALE = 2.0**127
 #: rows of a tile of the adapter kernels, and of the tiles that go through one kernel
 ADAPTER_ROWS, ADAPTER_FEW = 64, 16
 

@@ -550,7 +550,7 @@ int hds_adapter_parts(int n_tiles, int width);
  * of them sees the keys up to keys - new tokens + t, row tiles = ceil(new tokens * G / 8), units = (sequence, KV head, row tile) in this order;
  * workers int32 [n_workers][4] = (item, unit in it, first strip of 16 own keys in the unit, strips), consecutive pieces of the line of all
  * units' strips; units int32 [n_units][2] = (first, last worker); row_items int32 [rows] = the item of a row. Prefixes are whole pages ahead of the new
- * tokens. workspace: see below; nothing in it outlives the call. dtype 0 / 1. */
+ * tokens. scale: from 0 to below 2^127. workspace: see below; nothing in it outlives the call. dtype 0 / 1. */
 int hds_paged_attention_shared(const void* q, int64_t ld_q, void* out, int64_t ld_out, int rows, const void* kv_cache_layer, int64_t num_blocks,
                                const int32_t* block_tables, int max_blocks_per_seq, const int32_t* tiles, int n_tiles, int p_splits,
                                const int32_t* items, const int32_t* workers, int n_workers, const int32_t* units, int n_units,

@@ -8,6 +8,7 @@ import torch
 from hcache_deepspeed_b200.inference.sampling import LogitControls, sample_next
 from hcache_deepspeed_b200.linear import AdapterBank, MultiAdapterLinear
 from hcache_deepspeed_b200.ops import kernels, native, plans
+from hcache_deepspeed_b200.ops.backend import CpuOps
 
 
 # ---- the wrappers against a library that only notes its calls ------------------------------------------------------------
@@ -136,6 +137,19 @@ def test_sizes_that_the_library_takes_in_32_bits_are_refused_beyond(lib):
         with pytest.raises(ValueError, match="below 2.24"):
             kernels.adapter_add(**kw)
     assert not lib.calls
+
+
+@pytest.mark.parametrize("scale", [2.0**127, 3e38, 1e300, -1e-300])
+def test_scales_that_are_no_number_in_the_kernel_are_refused(lib, scale):
+    """Exponents are in powers of 2: 3e38 log2(e) is infinite in 32 bits, and infinity times a score of 0 is NaN."""
+    with pytest.raises(ValueError, match="scale"):
+        kernels.paged_attention_shared(**{**shared_call(), "scale": scale})
+    kw = shared_call()
+    with pytest.raises(ValueError, match="scale"):
+        CpuOps().attention_shared(*(kw[n].as_subclass(torch.Tensor) for n in ("q", "out", "kv_cache_layer", "block_tables")), kw["plan"], scale)
+    assert not lib.calls
+    kernels.paged_attention_shared(**{**shared_call(), "scale": 1.5e38})
+    assert lib.calls[-1][0] == "hds_paged_attention_shared"
 
 
 def test_the_package_imports_on_a_torch_without_cuda():
