@@ -16,6 +16,8 @@ OWN_ROWS, OWN_STRIP = 8, 16
 OWN_WORKERS, OWN_BEGIN = 12, 2
 #: microseconds: an SM's for a strip of own keys, a CTA's for 128 keys of a prefix under one and under two tiles of rows (measured, see attention_shared.cu)
 T_OWN, T_ONE, T_TWO = 0.17, 1.3, 2.9
+#: of a sequence: the kernels count to the end of its last tile in 32 bits
+MAX_KEYS = (1 << 31) - 129
 #: of attention's scores: times log2(e) it has to be a number in 32 bits
 MAX_SCALE = 2.0**127
 #: rows of a tile of the adapter kernels, and of the tiles that go through one kernel
@@ -99,8 +101,8 @@ class SharedPrefixPlan(_Plan):
             raise ValueError(f"{n_q_heads} query heads do not share {n_kv_heads} KV heads (up to 128 each)")
         if block_size not in (16, 32, 64, 128):
             raise ValueError("block_size must be 16, 32, 64 or 128")
-        if (new < 0).any() or (new > kv).any() or kv.size and int(kv.max()) >= 1 << 31:
-            raise ValueError("a sequence has at least its new tokens as keys, and fewer than 2^31")
+        if (new < 0).any() or (new > kv).any() or kv.size and int(kv.max()) > MAX_KEYS:
+            raise ValueError("a sequence has at least its new tokens as keys, and fewer than 2^31 - 128")
         self.n_q_heads, self.n_kv_heads, self.head_dim, self.block_size = n_q_heads, n_kv_heads, head_dim, block_size
         self.new_tokens, self.keys, self.groups = new, kv, [tuple(map(int, g)) for g in groups]
         self.n_seqs, self.rows = int(new.size), int(new.sum())

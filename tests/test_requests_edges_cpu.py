@@ -162,6 +162,17 @@ def test_the_package_imports_on_a_torch_without_cuda():
     assert done.returncode == 0, done.stderr[-2000:]
 
 
+# ---- plans ---------------------------------------------------------------------------------------------------------------
+def test_a_plan_leaves_room_behind_the_last_key():
+    """The kernels compare places up to a tile of 128 behind the last key with it, in 32 bits."""
+    with pytest.raises(ValueError, match="fewer than 2"):
+        plans.SharedPrefixPlan([1], [(1 << 31) - 128], [], 1, 1, 64, 16)
+    prefix = ((1 << 31) - 129) // 128 * 128
+    plan = plans.SharedPrefixPlan([1], [prefix + 2], [(0, 1, prefix)], 1, 1, 64, 128)
+    _, _, _, keys, prefix, _, _, _ = plan.items[0].tolist()
+    assert keys + 128 < 1 << 31 and -(-prefix // 128) * 128 < 1 << 31
+
+
 # ---- banks of adapters ---------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("convert", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.float16),
                                      lambda m: m.half().bfloat16()])
