@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from tests.test_gpu_requests import HALF, K, adapters_exact, adapters_inputs, attention_exact, check, pages, rand
+from tests.test_gpu_requests import (HALF, K, adapters_exact, adapters_inputs, attention_exact, check, controls_check, controls_exact, controls_inputs, pages,
+                                     rand)
 
 pytestmark = [pytest.mark.gpu, pytest.mark.timeout(300)]
 
@@ -64,3 +65,55 @@ def test_a_converted_bank_serves():
     ids, x = [1, -1, 0], rand(3, 64)
     y = layer(x, bank.plan(ids))
     check(y, *adapters_exact(K().gemm(x, layer.weight), x, bank.down, bank.up, bank.scales, ids))
+
+
+@pytest.mark.parametrize("dtype", HALF + [torch.float32])
+@pytest.mark.parametrize("n,V,cap,k", [(2, 1500, 40, 1400), (1, 3000, 5, 5000), (200, 300, 1500, 700)])
+def test_more_biases_than_a_chunk_keeps(dtype, n, V, cap, k):
+    """More than 512 of them in a chunk, of small and of large ones; of a token given twice the last one counts."""
+    logits, c = controls_inputs(n, V, dtype, cap, k, 1)
+    want, bound = controls_exact(logits, **c)
+    out = K().logit_controls(logits, **c)
+    controls_check(out, want, bound)
+    assert torch.equal(K().logit_controls(logits, logits, **c), out)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_a_grammar_that_changes_with_every_token(dtype):
+    from tests.test_requests_edges_cpu import check_grammar, tiny_engine
+    check_grammar(tiny_engine(dtype, "cuda"), "cuda")
+
+
+def test_sessions_decode_under_controls():
+    from tests.test_requests_edges_cpu import check_sessions_under_controls, tiny_engine
+    check_sessions_under_controls(tiny_engine(torch.bfloat16, "cuda"), "cuda")
+
+
+def test_generate_under_controls():
+    """On the GPU: a mask, a bias and penalties rule; a refused request leaves nothing; a session's second turn."""
+    transformers = pytest.importorskip("transformers")
+    import hcache_deepspeed_b200 as ds
+    torch.manual_seed(0)
+    cfg = transformers.LlamaConfig(vocab_size=512, hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                                   max_position_embeddings=512)
+    eng = ds.init_inference(transformers.LlamaForCausalLM(cfg).eval().to(torch.bfloat16).cuda(), dtype=torch.bfloat16, replace_with_kernel_inject=True,
+                            hcache={"max_context": 512, "max_batch_tokens": 256, "kv_memory_bytes": 64 << 20})
+    state = eng.ragged_engine.state_manager
+    free, tracked = int(state.free_blocks[0]), state.n_tracked_sequences
+    ids = torch.randint(3, 512, (2, 9)).cuda()
+    allowed = torch.zeros(2, 512, dtype=torch.bool)
+    allowed[0, 5] = allowed[1, 77] = True
+    assert eng.generate(input_ids=ids, max_new_tokens=3, allowed=allowed.cuda())[:, 9:].tolist() == [[5] * 3, [77] * 3]
+    odd = torch.ones(2, 512, dtype=torch.bool)
+    odd[:, ::2] = False
+    drawn = eng.generate(input_ids=ids, max_new_tokens=20, do_sample=True, allowed=odd, presence_penalty=-2.0)
+    assert (drawn[:, 9:] % 2 == 1).all()
+    every = eng.generate(input_ids=ids, max_new_tokens=30, presence_penalty=1e6)       # no token twice
+    assert all(len(set(row.tolist())) == len(row) for row in every[:, 9:])
+    with pytest.raises(ValueError):
+        eng.generate(input_ids=ids, max_new_tokens=3, logit_bias={512: 1.0})
+    assert (int(state.free_blocks[0]), state.n_tracked_sequences) == (free, tracked)
+    told = eng.generate(input_ids=ids, max_new_tokens=30, session_ids=[5, 6])
+    never = eng.generate(input_ids=told[:, -1:], max_new_tokens=30, session_ids=[5, 6], repetition_penalty=1e30)      # what was said has a logit of 0, or of -1e30
+    for a, b in zip(told, never):
+        assert not set(a.tolist()) & set(b[1:].tolist())

@@ -323,3 +323,94 @@ def test_controls_at_the_ends_of_32_bits():
     controls = LogitControls([[1, 2]], 4, 3, "cpu", repetition_penalty=3e38, presence_penalty=-1e-30, logit_bias={3: -1e39})
     assert controls.apply(torch.tensor([[1.0, 0.0, -1.0, 1.0]])).tolist() == [[1.0, 0.0, torch.tensor(-3e38).item(), float("-inf")]]
     assert sample_next(torch.tensor([[1.0, 0.0, -1.0, 1.0]]), controls=controls).tolist() == [0]
+
+
+def grammar_loop(engine, uids, prompts, controls, rule, steps, ends):
+    """A grammar that changes with every token: ``rule(token)`` is the set that may follow it. Sessions leave the batch at the token ``ends``."""
+    from hcache_deepspeed_b200.inference.sampling import sample_next
+    answers, alive = [[] for _ in uids], list(range(len(uids)))
+    logits, _ = engine.put(uids, prompts, capture_latents=False)
+    controls.set_allowed(torch.stack([rule(int(p[-1])) for p in prompts]))
+    for _ in range(steps):
+        tokens = sample_next(logits, controls=controls).tolist()
+        for i, tok in zip(alive, tokens):
+            answers[i].append(tok)
+        places = [j for j, tok in enumerate(tokens) if tok != ends]
+        if not places:
+            break
+        controls.keep(places)
+        alive, tokens = [alive[j] for j in places], [tokens[j] for j in places]
+        controls.set_allowed(torch.stack([rule(t) for t in tokens]))
+        logits, _ = engine.put([uids[i] for i in alive], [torch.tensor([t], dtype=torch.int32) for t in tokens], capture_latents=False)
+    return answers
+
+
+def tiny_engine(dtype=torch.float32, device="cpu"):
+    from hcache_deepspeed_b200.inference.v2 import RaggedInferenceEngineConfig, build_engine_from_arch
+    cfg = RaggedInferenceEngineConfig(state_manager=dict(max_tracked_sequences=16, max_ragged_batch_size=256, max_ragged_sequence_count=8, max_context=512,
+                                                         memory_config=dict(mode="allocate", size=32 << 20)), hcache={"enabled": True})
+    return build_engine_from_arch("tiny-llama-test", cfg, seed=1, dtype=dtype, device=torch.device(device))
+
+
+def check_grammar(engine, device):
+    """Tokens go up by 1 to 5 each, and 7 of a residue ends: every answer follows the rule, and has the penalties of its own history."""
+    V = engine.model().spec.vocab
+
+    def rule(token):
+        allowed = torch.zeros(V, dtype=torch.bool)
+        allowed[[(token + k) % V for k in range(1, 6)]] = True
+        allowed[V - 1] = token % 7 == 0          # the end
+        return allowed
+    prompts = [torch.tensor(p, dtype=torch.int32) for p in ([3, 9, 1], [4], [10, 20, 30, 7])]
+    controls = LogitControls(prompts, V, 12, device, presence_penalty=0.5, logit_bias={V - 1: 50.0})
+    answers = grammar_loop(engine, [1, 2, 3], prompts, controls, rule, 12, V - 1)
+    for p, answer in zip(prompts, answers):
+        before = int(p[-1])
+        for tok in answer:
+            assert rule(before)[tok]
+            before = tok
+        assert answer[-1] == V - 1 or len(answer) == 12
+        assert all((t == V - 1) == (b % 7 == 0) for b, t in zip([int(p[-1])] + answer, answer))       # (the bias takes the end where it is allowed)
+    assert answers[2] == [V - 1]
+
+
+def test_a_grammar_that_changes_with_every_token():
+    check_grammar(tiny_engine(), "cpu")
+
+
+def check_sessions_under_controls(engine, device):
+    """``HCacheSessionManager.decode`` of three sessions, one of which ends early, against drawing by hand."""
+    from hcache_deepspeed_b200.hcache import HCacheSessionManager
+    manager = HCacheSessionManager(engine, allow_recompute=False)
+    V = engine.model().spec.vocab
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, V, (n, ), generator=g).to(torch.int32) for n in (5, 9, 3)]
+    make = lambda: LogitControls(prompts, V, 8, device, repetition_penalty=[1.5, 3.0, 1.2], frequency_penalty=0.4, logit_bias=[{3: -9.0}, {}, {5: 2.0}])  # noqa: E731
+    uids = [11, 12, 13]
+    logits = torch.cat([manager.prefill(u, p).clone() for u, p in zip(uids, prompts)])
+    seen = []
+
+    def stop(uid, token):
+        seen.append((uid, token))
+        return uid == 12 and sum(u == 12 for u, _ in seen) == 3
+    answers = manager.decode(uids, 8, logits, stop=stop, controls=make())
+    assert [len(a) for a in answers] == [8, 3, 8]
+    for u in uids:
+        engine.flush(u)
+    controls, alive = make(), [0, 1, 2]
+    logits = torch.cat([engine.put([u], [p], capture_latents=False)[0].clone() for u, p in zip(uids, prompts)])
+    for step in range(8):
+        ruled = controls.apply(logits)
+        for j, i in enumerate(alive):
+            assert answers[i][step] == int(ruled[j].float().argmax())
+        tokens = torch.tensor([answers[i][step] for i in alive])
+        controls.append(tokens)
+        if step == 2:
+            alive = [0, 2]
+            controls.keep([0, 2])
+        if step < 7:
+            logits, _ = engine.put([uids[i] for i in alive], [torch.tensor([answers[i][step]], dtype=torch.int32) for i in alive], capture_latents=False)
+
+
+def test_sessions_decode_under_controls():
+    check_sessions_under_controls(tiny_engine(), "cpu")
