@@ -727,7 +727,7 @@ static int launch_shared(const CUtensorMap& tq, const CUtensorMap& tkv, const CU
     HDS_CHECK_CUDA(launch_kernel(parts, dim3(ctas), dim3(kSpThreads), sp_smem_bytes(D), s, tq, tkv, tstrip, a));
     const int64_t threads = static_cast<int64_t>(a.rows) * a.n_q_heads * (D / 4);
     // (as long as all CTAs find room at once: 6 per SM)
-    const int share = threads <= 148 * 6 * kJoinThreads / 4 ? 4 : threads <= 148 * 6 * kJoinThreads / 2 ? 2 : 1;
+    const int room = sm_count() * 6 * kJoinThreads, share = threads <= room / 4 ? 4 : threads <= room / 2 ? 2 : 1;
     HDS_CHECK_CUDA(launch_kernel(shared_join_kernel<D, kBf16>, dim3(static_cast<unsigned>((threads * share + kJoinThreads - 1) / kJoinThreads)), dim3(kJoinThreads), 0,
                                  s, a, share));
     return HDS_OK;

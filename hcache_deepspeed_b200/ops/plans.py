@@ -14,7 +14,8 @@ import torch
 OWN_ROWS, OWN_STRIP = 8, 16
 #: workers of a CTA for own keys; what beginning and end of a unit take, in strips
 OWN_WORKERS, OWN_BEGIN = 12, 2
-#: microseconds: an SM's for a strip of own keys, a CTA's for 128 keys of a prefix under one and under two tiles of rows (measured, see attention_shared.cu)
+#: weights of pick_shares, in microseconds: an SM's for a strip of own keys, a CTA's for 128 keys of a prefix under one and under two tiles of rows. Fitted to
+#: whole calls at an earlier state of the kernel, both parts running at once; a tile by itself takes less now (see attention_shared.cu)
 T_OWN, T_ONE, T_TWO = 0.17, 1.3, 2.9
 #: of a sequence: the kernels count to the end of its last tile in 32 bits
 MAX_KEYS = (1 << 31) - 129
@@ -137,10 +138,13 @@ class SharedPrefixPlan(_Plan):
         self.n_units, total = int(unit0[-1]), int(ends[-1])
         if total >= 1 << 31:
             raise ValueError("too many keys for one call")
+        self.device = None if device is None else torch.device(device)
+        on_gpu = self.device is not None and self.device.type == "cuda"
+        sms = [torch.cuda.get_device_properties(self.device).multi_processor_count] if on_gpu else []
         # a unit costs its strips and a beginning and end that take as long as OWN_BEGIN more
         costs = np.concatenate([[0], np.cumsum(np.where(strips[of_item] > 0, strips[of_item] + OWN_BEGIN, 0))])
         self.p_splits, ctas = pick_shares(self.n_tiles * n_kv_heads, max((t[3] for t in tiles), default=0),
-                                          any(t[2] > tile_tokens // 2 for t in tiles), int(costs[-1]))
+                                          any(t[2] > tile_tokens // 2 for t in tiles), int(costs[-1]), *sms)
         self.n_workers = W = min(ctas * OWN_WORKERS, -(-total // 2))
         cost = costs[-1] * np.arange(W + 1, dtype=np.int64) // max(W, 1)
         unit = np.searchsorted(costs, cost[:-1], side="right") - 1
@@ -152,10 +156,9 @@ class SharedPrefixPlan(_Plan):
         items[:, 0], items[:, 1], items[:, 2], items[:, 3] = np.arange(new.size), row0[:-1], new, kv
         items[:, 4], items[:, 5], items[:, 6] = prefix, unit0[:-1], row_tiles
         self.items, self.workers, self.units = items, workers.astype(np.int32), units.astype(np.int32)
-        self.device = None if device is None else torch.device(device)
         #: bytes of a call's scratch (0: the library has not been asked yet)
         self.workspace_bytes = 0
-        if self.device is not None and self.device.type == "cuda":
+        if on_gpu:
             row_items = np.repeat(np.arange(new.size), new).astype(np.int32)
             parts = [np.asarray(tiles, dtype=np.int32), items, self.workers, self.units, row_items]       # all but the last start on 16-byte boundaries
             flat = [np.concatenate([p.reshape(-1), np.zeros(-p.size % 4, dtype=np.int32)]) for p in parts]
@@ -165,7 +168,9 @@ class SharedPrefixPlan(_Plan):
 
 def pick_shares(units: int, prefix: int, two: bool, cost: int, sms: int = 148) -> Tuple[int, int]:
     """Parts of a prefix of that many tokens, ``units`` CTAs wide, and the CTAs for own keys of that cost in strips: both begin together, on SMs of
-    their own, and the later end counts. Within 5% of the best of 90 pairs at each of ten batches, where other pairs took up to twice as long."""
+    their own, and the later end counts. Measured at eleven batches beside 12 to 90 other pairs each (a third to three times the parts, half to twice the
+    CTAs): ten of them within 4% of the best pair, one 14% behind (36 units, prefix 10496, cost 1068: 33.3 us, and 29.2 with four parts for three); the
+    worst pairs took up to 2.3 times as long."""
     tiles = -(-prefix // 128)
     if units == 0 or tiles == 0:
         return 1, sms

@@ -173,6 +173,17 @@ def test_a_plan_leaves_room_behind_the_last_key():
     assert keys + 128 < 1 << 31 and -(-prefix // 128) * 128 < 1 << 31
 
 
+@pytest.mark.parametrize("sms", [20, 74, 148])
+def test_a_plan_deals_out_the_sms_that_its_device_has(monkeypatch, sms):
+    monkeypatch.setattr(torch.cuda, "get_device_properties", lambda device: type("P", (), {"multi_processor_count": sms}))
+    monkeypatch.setattr(plans._Plan, "_place", lambda self, flat, device: 0)
+    plan = plans.SharedPrefixPlan([1] * 20, [4096 + 300] * 20, [(0, 20, 4096)], 32, 8, 128, 64, device="cuda")
+    assert (plan.p_splits, -(-plan.n_workers // plans.OWN_WORKERS)) == plans.pick_shares(8, 4096, False, 20 * 8 * (19 + plans.OWN_BEGIN), sms)
+    assert plan.n_workers < sms * plans.OWN_WORKERS
+    alone = plans.SharedPrefixPlan([1] * 20, [4096 + 300] * 20, [], 32, 8, 128, 64, device="cuda")
+    assert alone.n_workers == sms * plans.OWN_WORKERS
+
+
 # ---- banks of adapters ---------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("convert", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.float16),
                                      lambda m: m.half().bfloat16()])
