@@ -179,7 +179,8 @@ class BlockedFlashAttn(DSKernelBase):
 
 class SharedPrefixAttn(DSKernelBase):
     """Causal attention of a batch whose sequences share prefixes, against the paged KV cache: each prefix is read once for its group
-    (``ops.plans.SharedPrefixPlan`` says which sequences share what). 16-bit, head sizes 64 and 128 on a GPU."""
+    (``ops.plans.SharedPrefixPlan`` says which sequences share what). 16-bit, head sizes 64 and 128 on a GPU. Pays where sequences x prefix is
+    some thousand keys or more, and up to about 64 new tokens per sequence; :class:`BlockedFlashAttn` serves the others faster."""
 
     def __init__(self, head_size: int, dtype: torch.dtype, scale: Optional[float] = None):
         self._check_dtype(dtype)

@@ -79,8 +79,8 @@ __device__ __forceinline__ const uint16_t* ad_row(const void* p, int row, int ld
 }
 
 // acc = 16 rows of x times NT * 8 rows of down (those from rb on), over the columns k0 to k1 in blocks of 32, of which this warp has number `b` and
-// every `step`-th after it. U of them are asked for at once: with fewer on the way the sum waits for memory (4099 rows x 4096, rank 32: 31.8 us
-// one by one). Rows of a tile that are not there repeat others, rows of down behind the rank the last ones: nobody looks at what they come to.
+// every `step`-th after it. U of them are asked for at once (rank 16, whole calls of 1 and 64 rows: 3.9 and 10.8 us one by one, 3.7 and 10.6 two,
+// 4.1 and 11.0 four). Rows of a tile that are not there repeat others, rows of down behind the rank the last ones: nobody looks at what they come to.
 // x1 may be x0.
 template <int NT, bool kBf16, int U>
 __device__ __forceinline__ void ad_down(float (&acc)[NT][4], const uint16_t* x0, const uint16_t* x1, const uint16_t* down, int rb, int rank, int width, int k0,
@@ -172,7 +172,9 @@ __device__ __forceinline__ void ad_copy(const AdapterArgs& a, const int4& tile, 
 }
 
 // (RANK: of these kernels, or 0 where it is only known when they run: with it addresses are constants and no step is half empty. 64 rows with 61
-// adapters, rank 16, 4096 -> 11008: 13.2 us without, 10.5 with it.)
+// adapters, 4096 -> 11008: 13.0 us without and 10.6 with it at rank 16, 18.2 and 14.1 at 32, 43.0 and 36.8 at 64. The powers of two whose sums fit the
+// registers in one go have kernels of their own, down to a whole step of the MMA. Others at the same rows: 12.5 us at rank 8, whose steps are half empty,
+// 17.8 at 24, 35.4 at 48, and 61 at 128 and 164 at 256, where x is read 2 and 4 times.)
 
 // ---- few rows --------------------------------------------------------------------------------------------------------------
 // Each warp has a ring of its own for its groups of 32 rows of `up` (contiguous: one bulk copy each), filled from the start on: 4 groups up to rank
