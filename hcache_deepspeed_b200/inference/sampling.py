@@ -101,6 +101,8 @@ class LogitControls:
         places = list(places)
         if places == list(range(self.n)):
             return
+        if any(not 0 <= p < self.n for p in places):       # (on a GPU the index itself would end the context)
+            raise ValueError(f"places {places} of {self.n} requests")
         at = torch.tensor(places, dtype=torch.int64, device=self.device)
         self._c = {name: t[at] for name, t in self._c.items()}
         self.n = len(places)

@@ -336,6 +336,18 @@ def test_controls_at_the_ends_of_32_bits():
     assert sample_next(torch.tensor([[1.0, 0.0, -1.0, 1.0]]), controls=controls).tolist() == [0]
 
 
+@pytest.mark.parametrize("places", [[3], [0, -1], [0, 1, 2, 3]])
+def test_requests_that_are_not_there_do_not_go_on(places):
+    controls = LogitControls([[1], [2], [3]], 9, 3, "cpu", 1.5)
+    with pytest.raises(ValueError, match="of 3 requests"):
+        controls.keep(places)
+    assert controls.n == 3
+    controls.keep([2, 0])
+    assert controls._c["history"][:, 0].tolist() == [3, 1]
+    with pytest.raises(ValueError, match="of 2 requests"):
+        controls.keep([2])
+
+
 def grammar_loop(engine, uids, prompts, controls, rule, steps, ends):
     """A grammar that changes with every token: ``rule(token)`` is the set that may follow it. Sessions leave the batch at the token ``ends``."""
     from hcache_deepspeed_b200.inference.sampling import sample_next
