@@ -110,10 +110,12 @@ class LogitControls:
 
 def _drawable(logits: torch.Tensor) -> torch.Tensor:
     """Logits whose softmax is a distribution whatever the controls left of them (drawing from anything else ends a GPU's context): an infinite one
-    is a very large one, and a row without any token has token 0, as the arg-max has it."""
-    x = torch.nan_to_num(logits.float(), nan=-math.inf, posinf=1e30, neginf=-math.inf)
+    is the largest there is, and a row without any token has token 0, as the arg-max has it. Rows whose largest logit may leave 32 bits when it is divided by
+    a temperature have it taken off."""
+    x = torch.nan_to_num(logits.float(), nan=-math.inf, posinf=torch.finfo(torch.float32).max, neginf=-math.inf)
     x[:, 0] = torch.where(x.amax(-1) == -math.inf, 0.0, x[:, 0])
-    return x
+    top = x.amax(-1, keepdim=True)
+    return x - torch.where(top.abs() > 1e30, top, 0.0)
 
 
 def sample_next(logits: torch.Tensor, do_sample: bool = False, temperature: float = 1.0, top_k: int = 0,

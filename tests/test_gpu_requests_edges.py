@@ -117,3 +117,8 @@ def test_generate_under_controls():
     never = eng.generate(input_ids=told[:, -1:], max_new_tokens=30, session_ids=[5, 6], repetition_penalty=1e30)      # what was said has a logit of 0, or of -1e30
     for a, b in zip(told, never):
         assert not set(a.tolist()) & set(b[1:].tolist())
+
+
+def test_drawing_far_out():
+    from tests.test_requests_edges_cpu import check_drawing_far_out
+    check_drawing_far_out("cuda")

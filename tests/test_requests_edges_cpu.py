@@ -5,7 +5,7 @@ import sys
 import pytest
 import torch
 
-from hcache_deepspeed_b200.inference.sampling import LogitControls, sample_next
+from hcache_deepspeed_b200.inference.sampling import LogitControls, _drawable, sample_next
 from hcache_deepspeed_b200.linear import AdapterBank, MultiAdapterLinear
 from hcache_deepspeed_b200.ops import kernels, native, plans
 from hcache_deepspeed_b200.ops.backend import CpuOps
@@ -346,6 +346,30 @@ def test_requests_that_are_not_there_do_not_go_on(places):
     assert controls._c["history"][:, 0].tolist() == [3, 1]
     with pytest.raises(ValueError, match="of 2 requests"):
         controls.keep([2])
+
+
+def check_drawing_far_out(device):
+    """Rows: a bias at the end of 32 bits; penalties that take everything there; two of them, of which one is larger; one token left that is far below;
+    infinities beside the largest number. Divided by a temperature below 1 these are infinite, and a softmax of them NaN, which a GPU's context
+    does not outlive."""
+    allowed = torch.ones(5, 6, dtype=torch.bool)
+    allowed[3] = torch.tensor([False, False, True, False, False, False])
+    bias = [{4: 3e38}, {v: -3.2e38 + 1e37 * v for v in range(6)}, {v: -3.4e38 + (v == 5) * 1e38 for v in range(6)}, {2: -3.4e38}, {1: 3.4e38}]
+    controls = LogitControls([[1]] * 5, 6, 12, device, logit_bias=bias, allowed=allowed)
+    logits = torch.zeros(5, 6, device=device)
+    logits[4, 3] = float("inf")
+    for kw in (dict(temperature=0.1), dict(temperature=1e-9), dict(temperature=0.5, top_k=2), dict(temperature=0.3, top_p=0.5), dict()):
+        assert sample_next(logits, do_sample=True, controls=controls, **kw).tolist() == [4, 5, 5, 2, 3], kw
+
+
+def test_drawing_far_out():
+    check_drawing_far_out("cpu")
+
+
+def test_ordinary_logits_are_drawn_as_they_are():
+    logits = torch.randn(7, 50) * 20
+    logits[2, 10:] = float("-inf")
+    assert torch.equal(_drawable(logits), logits)
 
 
 def grammar_loop(engine, uids, prompts, controls, rule, steps, ends):
