@@ -132,7 +132,9 @@ def sample_next(logits: torch.Tensor, do_sample: bool = False, temperature: floa
             from ..ops import kernels
             return kernels.argmax(logits.contiguous())
         return logits.float().argmax(-1).to(torch.int32)
-    x = logits.float() / max(temperature, 1e-6)
+    if math.isnan(temperature) or top_p < 0.0:       # (they would leave no distribution, and drawing from none ends a GPU's context)
+        raise ValueError(f"temperature is {temperature} and top_p {top_p}")
+    x = logits.float() / min(max(temperature, 1e-6), 1e30)       # (-inf stays that)
     if top_k and top_k > 0:
         kth = torch.topk(x, min(top_k, x.shape[-1]), dim=-1).values[..., -1:]
         x = x.masked_fill(x < kth, float("-inf"))

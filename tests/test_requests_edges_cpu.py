@@ -366,6 +366,19 @@ def test_drawing_far_out():
     check_drawing_far_out("cpu")
 
 
+def test_drawing_at_any_temperature():
+    logits, inf = torch.tensor([[1.0, -float("inf"), 2.0]] * 64), float("inf")
+    drawn = sample_next(logits, do_sample=True, temperature=inf).tolist()
+    assert set(drawn) == {0, 2}
+    controls = LogitControls([[1]] * 64, 3, 4, "cpu", allowed=torch.tensor([[True, True, False]] * 64))
+    assert sample_next(logits, do_sample=True, temperature=inf, controls=controls).tolist() == [0] * 64
+    assert sample_next(logits, do_sample=True, top_p=0.0).tolist() == [2] * 64
+    for kw in (dict(temperature=float("nan")), dict(top_p=-0.1)):
+        with pytest.raises(ValueError, match="temperature"):
+            sample_next(logits, do_sample=True, **kw)
+        sample_next(logits, **kw)       # nothing is drawn
+
+
 def test_ordinary_logits_are_drawn_as_they_are():
     logits = torch.randn(7, 50) * 20
     logits[2, 10:] = float("-inf")
