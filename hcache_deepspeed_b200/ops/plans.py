@@ -54,6 +54,16 @@ class _Plan:
             self._dev.record_stream(torch.cuda.current_stream(self.index))
             self._others = self._others | {stream}
 
+    # (a plan holds addresses: a copy's would outlive the memory behind them, and another process has none)
+    def __copy__(self):
+        return self
+
+    def __deepcopy__(self, memo):
+        return self
+
+    def __reduce__(self):
+        raise TypeError("a plan belongs to its process and device: make another one from its lists")
+
 
 class AdapterPlan(_Plan):
     """Which rows go through which adapter. ``ids[t]``: the adapter of row t, negative for none. ``device``: where the calls run (host

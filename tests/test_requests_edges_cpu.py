@@ -184,6 +184,17 @@ def test_a_plan_deals_out_the_sms_that_its_device_has(monkeypatch, sms):
     assert alone.n_workers == sms * plans.OWN_WORKERS
 
 
+@pytest.mark.parametrize("args", [adapters_call, shared_call])
+def test_copies_of_a_plan_are_the_plan(args):
+    """Its lists do not change, and a copy would have the addresses of memory that it does not hold."""
+    import copy
+    import pickle
+    plan = args()["plan"]
+    assert copy.copy(plan) is plan and copy.deepcopy({"plan": plan})["plan"] is plan
+    with pytest.raises(TypeError, match="process"):
+        pickle.dumps(plan)
+
+
 # ---- banks of adapters ---------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("convert", [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(), lambda m: m.to("cpu", torch.float16),
                                      lambda m: m.half().bfloat16()])
