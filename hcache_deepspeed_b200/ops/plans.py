@@ -61,8 +61,10 @@ class _Plan:
     def __deepcopy__(self, memo):
         return self
 
-    def __reduce__(self):
-        raise TypeError("a plan belongs to its process and device: make another one from its lists")
+    def __getstate__(self):
+        if self._dev is not None:
+            raise TypeError("a plan on a GPU belongs to its process: make another one from its lists")
+        return self.__dict__
 
 
 class AdapterPlan(_Plan):

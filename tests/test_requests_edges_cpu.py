@@ -193,6 +193,8 @@ def test_copies_of_a_plan_are_the_plan(args):
     assert copy.copy(plan) is plan and copy.deepcopy({"plan": plan})["plan"] is plan
     with pytest.raises(TypeError, match="process"):
         pickle.dumps(plan)
+    there = pickle.loads(pickle.dumps(plans.SharedPrefixPlan([1, 2], [40, 41], [(0, 2, 32)], 2, 2, 64, 16)))      # in host memory alone
+    assert there.index == -1 and there.rows == 3 and there.items.shape == (2, 8)
 
 
 # ---- banks of adapters ---------------------------------------------------------------------------------------------------
